@@ -47,12 +47,17 @@ extern "C" {
 #define LS_DEVERR_TIMEOUT 0x1          /* a bounded wait expired; outputs are invalid */
 #define LS_DEVERR_PAGE_INDEX 0x2       /* a topk_idx entry >= number of key pages (ignored) */
 #define LS_DEVERR_SEQLENS 0x4          /* cu_seqlens not monotone or beyond the totals */
+#define LS_DEVERR_PAGES 0x8            /* ls_plan_pages ran out of free pages */
 
 /* Largest per-row page budget T accepted by ls_select_pages/ls_sparse_attn. */
 #define LS_MAX_TOPK 128
 
 /* Most page-list slices per row accepted by ls_sparse_attn_split. */
 #define LS_MAX_ATTN_SPLITS 64
+
+/* Tokens per page of the 8-bit paged cache, and most requests per ls_plan_pages. */
+#define LS_PAGE_TOKENS 64
+#define LS_MAX_PLAN_BATCH 8192
 
 /* Human-readable name of an LS_ERR_* code. */
 const char* ls_status_string(int code);
@@ -398,6 +403,92 @@ int ls_sparse_attn_gather_only(const uint16_t* q, const uint16_t* k, const uint1
                                int32_t num_kv_heads, int32_t head_dim, const int32_t* topk_idx,
                                int32_t topk, int32_t block_size, int32_t causal, int32_t* status,
                                void* stream);
+
+/*
+ * The 8-bit paged key/value cache (no reference counterpart: the reference
+ * decodes over a bf16 cache of packed rows).  A page holds 64 tokens of every
+ * KV head: k_pages and v_pages [num_pages, G, 64, 128] e4m3 codes, k_scale
+ * and v_scale [num_pages, G] fp32; a key is its code times the scale of its
+ * (page, head).  A request's pages are listed in block_table [batch,
+ * max_blocks] (entry j: the page of its tokens 64 j .. 64 j + 63, -1 when it
+ * has none).  One step of a batch is ls_plan_pages, ls_append_kv per layer
+ * and ls_paged_attn per layer.
+ */
+
+/*
+ * ls_plan_pages -- pages, slots and positions of one step.  Request b holds
+ * context_lens[b] tokens and adds new_lens[b] (>= 0); its tokens are packed
+ * one request after the other.  Writes
+ *   seq_lens [batch]         context + new tokens
+ *   cu_seqlens_q [batch+1]   prefix sums of new_lens
+ *   cu_blocks [batch+1]      prefix sums of the pages each request writes
+ *   positions [total_new]    a token's position in its request
+ *   slots [total_new]        page * 64 + position % 64, -1 without a page
+ *   block_table              the entries of blocks that begin in this step:
+ *                            free_pages[*free_head ...] in request order
+ *   free_head_out [1]        *free_head + pages taken (at most num_free); not
+ *                            the free_head buffer itself
+ * so the same call made twice gives the same results, and the next step
+ * passes seq_lens and free_head_out on.  total_new is the packed row count the
+ * caller knows; rows behind the last request get slot -1, position 0.  When
+ * the pages run out the entries stay -1 and LS_DEVERR_PAGES is raised;
+ * negative lengths, requests beyond max_blocks pages (their tokens get slot
+ * -1) and more tokens than total_new (not planned) raise LS_DEVERR_SEQLENS.
+ * batch <= LS_MAX_PLAN_BATCH.
+ */
+int ls_plan_pages(const int32_t* context_lens, const int32_t* new_lens, int32_t batch,
+                  int32_t* block_table, int32_t max_blocks, const int32_t* free_pages,
+                  int32_t num_free, const int32_t* free_head, int64_t total_new,
+                  int32_t* seq_lens, int32_t* cu_seqlens_q, int32_t* cu_blocks, int64_t* slots,
+                  int64_t* positions, int32_t* free_head_out, int32_t* status, void* stream);
+
+/*
+ * ls_append_kv -- rounds the planned step's k and v [total_new, G, 128] bf16
+ * into their pages.  Heads are contiguous, tokens k_stride / v_stride elements
+ * apart (multiples of 8: views of a fused projection need no copy).  For each
+ * (page, head) written, K and V apart: the scale becomes the smallest power
+ * of two s = 2^e, -40 <= e <= 48, with |x| <= 448 s for the page's new rows,
+ * and is never lowered while the page holds older tokens, whose codes are
+ * rescaled when it grows; codes are x / s rounded to the nearest e4m3 value
+ * (ties to even, saturating; NaN stays NaN and does not count for s).  Rows
+ * of a page behind the request's last token are left as they were, tokens
+ * with slot -1 are not stored.  A page written here must belong to one
+ * request only.
+ */
+int ls_append_kv(const uint16_t* k, const uint16_t* v, int64_t k_stride, int64_t v_stride,
+                 int64_t total_new, int32_t batch, int32_t num_kv_heads, int32_t head_dim,
+                 const int32_t* context_lens, const int32_t* seq_lens, const int32_t* cu_seqlens_q,
+                 const int32_t* cu_blocks, const int64_t* slots, uint8_t* k_pages,
+                 uint8_t* v_pages, float* k_scale, float* v_scale, int64_t num_pages,
+                 int32_t* status, void* stream);
+
+/*
+ * ls_paged_attn -- attention of packed query rows over the paged cache, the
+ * counterpart of ls_sparse_attn with an 8-bit cache.  Query row i of request
+ * b (rows cu_seqlens_q[b] .. cu_seqlens_q[b+1], nq of them) stands at position
+ * seq_lens[b] - nq + i: the step's own tokens are already in the cache.
+ *   out[t, h] = softmax_k(scale * q[t,h]·k[k,g]) v[k,g],  g = h / (H/G)
+ * over the request's keys in pages topk_idx[g, t, :] ([G, total_q, topk]
+ * block numbers of the request, < 0 empty, duplicates count once), or in all
+ * its pages when topk == 0, and with causal != 0 at positions up to the row's.
+ * Rows with no key output zeros (lse = +inf); rows behind the last request
+ * are left as they were.  Scales are read clamped to [2^-40, 2^48].  q and
+ * out [total_q, H, 128] bf16, lse [H, total_q] fp32 (nullable); scale <= 0
+ * selects 128^-0.5.  Requires 1 <= H/G <= 16, topk <= LS_MAX_TOPK.
+ * max_seqlen_q / max_seqlen_k bound nq and seq_lens.  `workspace` (16-byte
+ * aligned) holds ls_paged_attn_workspace_bytes() bytes; calls that may overlap
+ * need one each.  Block-table entries outside [0, num_pages) and list entries
+ * past the request's pages are passed over (LS_DEVERR_PAGE_INDEX).
+ */
+size_t ls_paged_attn_workspace_bytes(void);
+int ls_paged_attn(const uint16_t* q, const uint8_t* k_pages, const uint8_t* v_pages,
+                  const float* k_scale, const float* v_scale, int64_t num_pages,
+                  const int32_t* block_table, int32_t max_blocks, const int32_t* seq_lens,
+                  const int32_t* cu_seqlens_q, int32_t batch, int32_t max_seqlen_q,
+                  int32_t max_seqlen_k, int64_t total_q, int32_t num_heads, int32_t num_kv_heads,
+                  int32_t head_dim, const int32_t* topk_idx, int32_t topk, float softmax_scale,
+                  int32_t causal, void* workspace, size_t workspace_bytes, uint16_t* out,
+                  float* lse, int32_t* status, void* stream);
 
 /*
  * ls_wait_timeout_probe -- test hook for the bounded waits (no reference

@@ -64,6 +64,21 @@ bool make_tensor_map_2d(CUtensorMap* map, const void* base, uint64_t rows, uint6
   return res == CUDA_SUCCESS;
 }
 
+bool make_tensor_map_2d_u8(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols,
+                           uint32_t box_cols, uint32_t box_rows) {
+  auto encode = get_encode_fn();
+  if (encode == nullptr) return false;
+  cuuint64_t dims[2] = {cols, rows};
+  cuuint64_t strides[1] = {cols};
+  cuuint32_t box[2] = {box_cols, box_rows};
+  cuuint32_t elem_strides[2] = {1, 1};
+  const CUresult res = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims,
+                              strides, box, elem_strides, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return res == CUDA_SUCCESS;
+}
+
 int set_host_error(int code, const char* message) { return fail(code, "%s", message); }
 
 }  // namespace ls
@@ -702,6 +717,184 @@ int ls_sparse_attn_gather_only(const uint16_t* q, const uint16_t* k, const uint1
   return sparse_attn_impl(q, k, v, cu_seqlens_q, cu_seqlens_k, batch, max_seqlen_q, max_seqlen_k,
                           total_q, total_k, num_heads, num_kv_heads, head_dim, topk_idx, topk,
                           block_size, 0.f, causal, nullptr, nullptr, status, stream, true);
+}
+
+// ---------------------------------------------------------------------------
+// The 8-bit paged cache
+// ---------------------------------------------------------------------------
+
+int ls_plan_pages(const int32_t* context_lens, const int32_t* new_lens, int32_t batch,
+                  int32_t* block_table, int32_t max_blocks, const int32_t* free_pages,
+                  int32_t num_free, const int32_t* free_head, int64_t total_new,
+                  int32_t* seq_lens, int32_t* cu_seqlens_q, int32_t* cu_blocks, int64_t* slots,
+                  int64_t* positions, int32_t* free_head_out, int32_t* status, void* stream) {
+  LS_REQUIRE(context_lens && new_lens && block_table && free_head, "null argument");
+  LS_REQUIRE(seq_lens && cu_seqlens_q && cu_blocks && free_head_out, "null output");
+  LS_REQUIRE(free_head != free_head_out, "free_head_out must not be free_head");
+  LS_REQUIRE(batch >= 1 && max_blocks >= 1 && num_free >= 0, "bad sizes");
+  LS_REQUIRE(num_free == 0 || free_pages, "null free_pages");
+  LS_REQUIRE(total_new >= 0 && total_new < (int64_t{1} << 31), "total_new out of range");
+  LS_REQUIRE(total_new == 0 || (slots && positions), "null slots or positions");
+  if (batch > LS_MAX_PLAN_BATCH)
+    return fail(LS_ERR_UNSUPPORTED, "batch exceeds LS_MAX_PLAN_BATCH");
+  PlanArgs a{};
+  a.context_lens = context_lens;
+  a.new_lens = new_lens;
+  a.batch = batch;
+  a.block_table = block_table;
+  a.max_blocks = max_blocks;
+  a.free_pages = free_pages;
+  a.num_free = num_free;
+  a.free_head = free_head;
+  a.total_new = total_new;
+  a.seq_lens = seq_lens;
+  a.cu_seqlens_q = cu_seqlens_q;
+  a.cu_blocks = cu_blocks;
+  a.slots = slots;
+  a.positions = positions;
+  a.free_head_out = free_head_out;
+  a.status = status;
+  const cudaError_t err = launch_plan_pages(a, static_cast<cudaStream_t>(stream));
+  return err == cudaSuccess ? LS_OK : cuda_fail(err, "plan_pages launch");
+}
+
+namespace {
+
+int check_cache(const uint8_t* k_pages, const uint8_t* v_pages, const float* k_scale,
+                const float* v_scale, int64_t num_pages, int32_t num_kv_heads, int32_t head_dim) {
+  LS_REQUIRE(k_pages && v_pages && k_scale && v_scale, "null cache");
+  LS_REQUIRE(num_pages >= 1 && num_kv_heads >= 1 && num_kv_heads <= 65535, "bad cache sizes");
+  // Pages are addressed as rows of 128 bytes by 32-bit TMA coordinates.
+  LS_REQUIRE(num_pages * num_kv_heads < (int64_t{1} << 31) / LS_PAGE_TOKENS,
+             "num_pages * num_kv_heads out of range");
+  if (head_dim != 128) return fail(LS_ERR_UNSUPPORTED, "head_dim must be 128");
+  LS_REQUIRE_ALIGNED(k_pages);
+  LS_REQUIRE_ALIGNED(v_pages);
+  return LS_OK;
+}
+
+}  // namespace
+
+int ls_append_kv(const uint16_t* k, const uint16_t* v, int64_t k_stride, int64_t v_stride,
+                 int64_t total_new, int32_t batch, int32_t num_kv_heads, int32_t head_dim,
+                 const int32_t* context_lens, const int32_t* seq_lens, const int32_t* cu_seqlens_q,
+                 const int32_t* cu_blocks, const int64_t* slots, uint8_t* k_pages,
+                 uint8_t* v_pages, float* k_scale, float* v_scale, int64_t num_pages,
+                 int32_t* status, void* stream) {
+  const int rc = check_cache(k_pages, v_pages, k_scale, v_scale, num_pages, num_kv_heads, head_dim);
+  if (rc != LS_OK) return rc;
+  LS_REQUIRE(batch >= 1 && total_new >= 0 && total_new < (int64_t{1} << 31), "bad sizes");
+  if (total_new == 0) return LS_OK;
+  LS_REQUIRE(k && v && context_lens && seq_lens && cu_seqlens_q && cu_blocks && slots,
+             "null argument");
+  const int64_t row = static_cast<int64_t>(num_kv_heads) * 128;
+  LS_REQUIRE(k_stride >= row && v_stride >= row, "token strides overlap the heads");
+  if (k_stride % 8 != 0 || v_stride % 8 != 0)
+    return fail(LS_ERR_ALIGNMENT, "token strides must be multiples of 8 elements");
+  LS_REQUIRE_ALIGNED(k);
+  LS_REQUIRE_ALIGNED(v);
+  AppendArgs a{};
+  a.k = k;
+  a.v = v;
+  a.k_stride = k_stride;
+  a.v_stride = v_stride;
+  a.total_new = total_new;
+  a.batch = batch;
+  a.num_groups = num_kv_heads;
+  a.context_lens = context_lens;
+  a.seq_lens = seq_lens;
+  a.cu_seqlens_q = cu_seqlens_q;
+  a.cu_blocks = cu_blocks;
+  a.slots = slots;
+  a.k_pages = k_pages;
+  a.v_pages = v_pages;
+  a.k_scale = k_scale;
+  a.v_scale = v_scale;
+  a.num_pages = num_pages;
+  a.status = status;
+  const cudaError_t err = launch_append_kv(a, static_cast<cudaStream_t>(stream));
+  return err == cudaSuccess ? LS_OK : cuda_fail(err, "append_kv launch");
+}
+
+namespace {
+// Bytes of one CTA's share of the paged attention workspace: the header, two
+// partial rows of 16 heads (128 sums, row reference and row sum).
+constexpr size_t kPagedPartFloats = 16 * (128 + 2);
+constexpr size_t kPagedCtaBytes = 16 + 2 * kPagedPartFloats * sizeof(float);
+}  // namespace
+
+size_t ls_paged_attn_workspace_bytes(void) { return kPagedMaxCtas * kPagedCtaBytes; }
+
+int ls_paged_attn(const uint16_t* q, const uint8_t* k_pages, const uint8_t* v_pages,
+                  const float* k_scale, const float* v_scale, int64_t num_pages,
+                  const int32_t* block_table, int32_t max_blocks, const int32_t* seq_lens,
+                  const int32_t* cu_seqlens_q, int32_t batch, int32_t max_seqlen_q,
+                  int32_t max_seqlen_k, int64_t total_q, int32_t num_heads, int32_t num_kv_heads,
+                  int32_t head_dim, const int32_t* topk_idx, int32_t topk, float softmax_scale,
+                  int32_t causal, void* workspace, size_t workspace_bytes, uint16_t* out,
+                  float* lse, int32_t* status, void* stream) {
+  const int rc = check_cache(k_pages, v_pages, k_scale, v_scale, num_pages, num_kv_heads, head_dim);
+  if (rc != LS_OK) return rc;
+  LS_REQUIRE(q && block_table && seq_lens && cu_seqlens_q && out, "null argument");
+  LS_REQUIRE(batch >= 1 && max_blocks >= 1 && total_q >= 0, "bad sizes");
+  LS_REQUIRE(max_blocks <= (1 << 24), "max_blocks out of range");
+  LS_REQUIRE(max_seqlen_q >= 0 && max_seqlen_k >= 0, "bad max_seqlen");
+  LS_REQUIRE(num_heads > 0 && num_heads % num_kv_heads == 0,
+             "num_heads must be a positive multiple of num_kv_heads");
+  LS_REQUIRE(total_q * num_kv_heads < (int64_t{1} << 31), "num_kv_heads * total_q out of range");
+  LS_REQUIRE(topk >= 0 && (topk == 0 || topk_idx), "null topk_idx");
+  if (topk > LS_MAX_TOPK) return fail(LS_ERR_UNSUPPORTED, "topk exceeds LS_MAX_TOPK");
+  const int hg = num_heads / num_kv_heads;
+  if (hg > 16) return fail(LS_ERR_UNSUPPORTED, "heads per group must be at most 16");
+  LS_REQUIRE_ALIGNED(q);
+  LS_REQUIRE_ALIGNED(out);
+  if (total_q == 0) return LS_OK;
+  const size_t need = ls_paged_attn_workspace_bytes();
+  LS_REQUIRE(workspace && workspace_bytes >= need, "workspace too small: %zu < %zu bytes",
+             workspace_bytes, need);
+  LS_REQUIRE_ALIGNED(workspace);
+  int device = 0, sms = 0;
+  cudaError_t err = cudaGetDevice(&device);
+  if (err == cudaSuccess)
+    err = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
+  if (err != cudaSuccess) return cuda_fail(err, "device query");
+  PagedAttnArgs a{};
+  const uint64_t rows = static_cast<uint64_t>(num_pages) * num_kv_heads * LS_PAGE_TOKENS;
+  if (!make_tensor_map_2d_u8(&a.tm_k, k_pages, rows, 128, 128, LS_PAGE_TOKENS))
+    return fail(LS_ERR_CUDA, "cuTensorMapEncodeTiled failed for k_pages");
+  if (!make_tensor_map_2d_u8(&a.tm_v, v_pages, rows, 128, 128, LS_PAGE_TOKENS))
+    return fail(LS_ERR_CUDA, "cuTensorMapEncodeTiled failed for v_pages");
+  a.q = q;
+  a.k_scale = k_scale;
+  a.v_scale = v_scale;
+  a.num_pages = num_pages;
+  a.block_table = block_table;
+  a.max_blocks = max_blocks;
+  a.seq_lens = seq_lens;
+  a.cu_q = cu_seqlens_q;
+  a.batch = batch;
+  a.total_q = total_q;
+  a.num_heads = num_heads;
+  a.num_groups = num_kv_heads;
+  a.heads_per_group = hg;
+  a.topk_idx = topk_idx;
+  a.topk = topk;
+  a.causal = causal;
+  const float scale = softmax_scale > 0.f ? softmax_scale : 0.08838834764831845f;  // 128^-0.5
+  a.scale_log2 = scale * 1.4426950408889634f;
+  a.out = out;
+  a.lse = lse;
+  a.headers = static_cast<int2*>(workspace);
+  a.part_ml = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kPagedMaxCtas * 16);
+  a.part_o = a.part_ml + 2 * kPagedMaxCtas * 16 * 2;
+  a.status = status;
+  // At most one CTA per scheduled page: the caller's max_seqlen_k bounds the
+  // pages of a dense row (a longer request only gets fewer CTAs).
+  const int64_t per_row = topk > 0 ? topk : std::max<int64_t>(1, (int64_t{max_seqlen_k} + 63) / 64);
+  const int64_t want = total_q * num_kv_heads * per_row;
+  const int ctas = static_cast<int>(std::min<int64_t>({want, 2 * sms, kPagedMaxCtas}));
+  err = launch_paged_attn(a, ctas, static_cast<cudaStream_t>(stream));
+  return err == cudaSuccess ? LS_OK : cuda_fail(err, "paged_attn launch");
 }
 
 }  // extern "C"

@@ -126,6 +126,84 @@ cudaError_t launch_sparse_attn_merge(const AttnArgs& args, cudaStream_t stream);
 // the attention kernel cannot beat (a measured roofline for it).
 cudaError_t launch_sparse_attn_gather_only(const AttnArgs& args, cudaStream_t stream);
 
+// Page planning and cache write of the 8-bit paged cache (paged_cache.cu).
+struct PlanArgs {
+  const int32_t* context_lens;
+  const int32_t* new_lens;
+  int batch;
+  int32_t* block_table;   // [batch, max_blocks]
+  int max_blocks;
+  const int32_t* free_pages;
+  int num_free;
+  const int32_t* free_head;
+  int64_t total_new;
+  int32_t* seq_lens;
+  int32_t* cu_seqlens_q;
+  int32_t* cu_blocks;
+  int64_t* slots;
+  int64_t* positions;
+  int32_t* free_head_out;
+  int32_t* status;
+};
+
+cudaError_t launch_plan_pages(const PlanArgs& args, cudaStream_t stream);
+
+struct AppendArgs {
+  const uint16_t* k;
+  const uint16_t* v;
+  int64_t k_stride;       // elements between tokens
+  int64_t v_stride;
+  int64_t total_new;
+  int batch;
+  int num_groups;
+  const int32_t* context_lens;
+  const int32_t* seq_lens;
+  const int32_t* cu_seqlens_q;
+  const int32_t* cu_blocks;
+  const int64_t* slots;
+  uint8_t* k_pages;       // [num_pages, num_groups, 64, 128] e4m3
+  uint8_t* v_pages;
+  float* k_scale;         // [num_pages, num_groups]
+  float* v_scale;
+  int64_t num_pages;
+  int32_t* status;
+};
+
+cudaError_t launch_append_kv(const AppendArgs& args, cudaStream_t stream);
+
+// Attention over the paged cache (paged_attn.cu).
+constexpr int kPagedMaxCtas = 2 * 148;  // two resident CTAs on each of the B200's SMs
+
+struct PagedAttnArgs {
+  CUtensorMap tm_k;       // K codes as [num_pages * G * 64, 128] bytes, box {128, 64}, 128B swizzle
+  CUtensorMap tm_v;
+  const uint16_t* q;
+  const float* k_scale;
+  const float* v_scale;
+  int64_t num_pages;
+  const int32_t* block_table;
+  int max_blocks;
+  const int32_t* seq_lens;
+  const int32_t* cu_q;
+  int batch;
+  int64_t total_q;
+  int num_heads;
+  int num_groups;
+  int heads_per_group;    // 1 .. 16
+  const int32_t* topk_idx;  // [G, total_q, topk], topk == 0: every page of the request
+  int topk;
+  int causal;
+  float scale_log2;       // softmax_scale * log2(e)
+  uint16_t* out;
+  float* lse;
+  int2* headers;          // workspace: per CTA, the row it leaves unfinished and that row's last CTA
+  float* part_ml;         // [2 * CTAs, 16, 2]: row reference (log2) and row sum
+  float* part_o;          // [2 * CTAs, 16, 128]
+  int32_t* status;
+};
+
+cudaError_t launch_paged_attn(const PagedAttnArgs& args, int ctas, cudaStream_t stream);
+
 // Host-side argument checks of ls_select_pages other than its workspace
 // (shared with ls_select_pages_noalloc); LS_OK or the LS_ERR_* code it sets.
 int check_select_args(const uint16_t* q, const uint16_t* wq_t, const uint16_t* ks,
@@ -146,5 +224,9 @@ int set_host_error(int code, const char* message);
 // Returns false if the driver entry point is unavailable or encoding fails.
 bool make_tensor_map_2d(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols,
                         uint64_t row_stride_bytes, uint32_t box_cols, uint32_t box_rows);
+
+// The same for 8-bit elements and contiguous rows.
+bool make_tensor_map_2d_u8(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols,
+                           uint32_t box_cols, uint32_t box_rows);
 
 }  // namespace ls

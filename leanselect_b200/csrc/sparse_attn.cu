@@ -27,6 +27,7 @@
 // partial results that attn_merge_kernel combines.
 #include "common.cuh"
 #include "launch.h"
+#include "page_list.cuh"
 
 namespace ls {
 namespace {
@@ -36,7 +37,6 @@ constexpr int kBoxBytes = 64 * 128;            // 64 keys x 64 dims bf16
 constexpr int kStageBytes = 4 * kBoxBytes;     // K half0, K half1, V half0, V half1
 constexpr int kThreads = 160;
 constexpr int kMaxT = LS_MAX_TOPK;
-constexpr int32_t kSentinel = 0x7FFFFFFF;
 constexpr float kRescaleSlack = 8.f;  // log2 units: exponentials stay below 256
 
 struct AttnSmem {
@@ -81,40 +81,6 @@ __device__ __forceinline__ float ex2(float x) {
 // Byte offset of 16-byte chunk `chunk` (0..7) of row `row` in a 128B-swizzled box.
 __device__ __forceinline__ uint32_t sw128(int row, int chunk) {
   return static_cast<uint32_t>(row * 128 + ((chunk ^ (row & 7)) << 4));
-}
-
-// Sorts 128 keys held as v[r] at position 32*r + lane, ascending.
-__device__ __forceinline__ void warp_bitonic_sort128(int32_t (&v)[4], int lane) {
-#pragma unroll
-  for (int k = 2; k <= 128; k <<= 1) {
-#pragma unroll
-    for (int j = k >> 1; j > 0; j >>= 1) {
-      if (j >= 32) {
-        const int rj = j >> 5;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          if ((r & rj) == 0) {
-            const int pos = 32 * r + lane;
-            const bool up = (pos & k) == 0;
-            const int32_t a = v[r], b = v[r | rj];
-            const bool swap = up ? (a > b) : (a < b);
-            v[r] = swap ? b : a;
-            v[r | rj] = swap ? a : b;
-          }
-        }
-      } else {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int pos = 32 * r + lane;
-          const int32_t other = __shfl_xor_sync(0xffffffffu, v[r], j);
-          const bool up = (pos & k) == 0;
-          const bool lower = (lane & j) == 0;
-          const int32_t lo = min(v[r], other), hi = max(v[r], other);
-          v[r] = (lower == up) ? lo : hi;
-        }
-      }
-    }
-  }
 }
 
 template <int HG, bool kGatherOnly>
@@ -182,31 +148,10 @@ __global__ void __launch_bounds__(kThreads, 2) sparse_attn_kernel(const __grid_c
     for (int r = 0; r < 4; ++r) {
       const int32_t p = praw[r];
       if (p >= n_kpages) bad_index = true;
-      v[r] = (p >= 0 && p < n_kpages && p * 64 <= t_lim) ? p : kSentinel;
+      v[r] = (p >= 0 && p < n_kpages && p * 64 <= t_lim) ? p : kPageSentinel;
     }
     if (__any_sync(0xffffffffu, bad_index) && lane == 0) report(args.status, LS_DEVERR_PAGE_INDEX);
-    // Strictly ascending valid entries followed by sentinels (the lists the
-    // selection kernels write) need no sort.
-    bool ordered = true;
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      int32_t next = __shfl_down_sync(0xffffffffu, v[r], 1);
-      const int32_t next_row = __shfl_sync(0xffffffffu, v[r < 3 ? r + 1 : r], 0);
-      if (lane == 31) next = r < 3 ? next_row : kSentinel;
-      ordered = ordered && (v[r] < next || next == kSentinel);
-    }
-    if (!__all_sync(0xffffffffu, ordered)) warp_bitonic_sort128(v, lane);
-    int base = 0;
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      int32_t prev = __shfl_up_sync(0xffffffffu, v[r], 1);
-      const int32_t prev_reg = r > 0 ? __shfl_sync(0xffffffffu, v[r - 1], 31) : -1;
-      if (lane == 0) prev = prev_reg;
-      const bool keep = v[r] != kSentinel && v[r] != prev;
-      const uint32_t mask = __ballot_sync(0xffffffffu, keep);
-      if (keep) sm->pages[base + __popc(mask & ((1u << lane) - 1))] = v[r];
-      base += __popc(mask);
-    }
+    const int base = warp_compact_pages(v, sm->pages, lane);
     if (lane == 0) sm->n_pages = base;
   } else if (warp == 1) {
     // Q rows of this group (HG heads, padded to 16 rows with zeros), swizzled.

@@ -76,7 +76,8 @@ def check_status(device: torch.device | int | None = None, reset: bool = True) -
     if bits:
         names = [n for n, b in (("TIMEOUT", _native.LS_DEVERR_TIMEOUT),
                                 ("PAGE_INDEX", _native.LS_DEVERR_PAGE_INDEX),
-                                ("SEQLENS", _native.LS_DEVERR_SEQLENS)) if bits & b]
+                                ("SEQLENS", _native.LS_DEVERR_SEQLENS),
+                                ("PAGES", _native.LS_DEVERR_PAGES)) if bits & b]
         raise LeanSelectError(-bits, f"device status bits set: {'|'.join(names)}")
     return bits
 
@@ -560,3 +561,178 @@ def sparse_attn_gather_only(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                cu_q.data_ptr(), cu_k.data_ptr(), cu_q.numel() - 1, int(max_seqlen_q),
                int(max_seqlen_k), total_q, total_k, H, G, D, idx.data_ptr(), idx.shape[2],
                block_size, 1 if causal else 0, status_word(dev).data_ptr(), _stream(dev))
+
+
+# ---------------------------------------------------------------------------
+# the 8-bit paged key/value cache
+# ---------------------------------------------------------------------------
+
+@dataclass
+class PagePlan:
+    """One step of a batch over the paged cache (:func:`plan_pages`)."""
+
+    context_lens: torch.Tensor   # [B] int32, tokens cached before the step
+    seq_lens: torch.Tensor       # [B] int32, with the step's tokens
+    cu_seqlens_q: torch.Tensor   # [B+1] int32, the step's packed rows
+    cu_blocks: torch.Tensor      # [B+1] int32, pages each request writes
+    slots: torch.Tensor          # [total_new] int64, page * 64 + offset (-1: no page)
+    positions: torch.Tensor      # [total_new] int64
+    free_head: torch.Tensor | None = None  # [1] int32, the free list after the step
+
+
+def _exact_tensor(t: torch.Tensor, name: str, dtype: torch.dtype, shape) -> None:
+    """A tensor the kernels use in place: its own type and layout, no copies."""
+    if t.dtype != dtype:
+        raise ValueError(f"{name} must be {dtype}, not {t.dtype}")
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} must have shape {tuple(shape)}, not {tuple(t.shape)}")
+    if not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+
+
+def plan_pages(context_lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch.Tensor,
+               free_pages: torch.Tensor, free_head: torch.Tensor, total_new: int) -> PagePlan:
+    """Pages, slots and positions of one step, on the GPU (``ls_plan_pages``).
+
+    Request ``b`` holds ``context_lens[b]`` tokens and adds ``new_lens[b]``.
+    Blocks that begin in this step take the next entries of ``free_pages``
+    behind ``free_head [1]``; ``block_table [B, max_blocks]`` is updated in
+    place.  ``total_new`` is the packed row count the caller knows (rows behind
+    the last request get slot -1).  The next step passes ``plan.seq_lens`` and
+    ``plan.free_head`` on; nothing here reads the device back.
+    """
+    dev = _require_cuda(context_lens, new_lens, block_table, free_pages, free_head)
+    ctx, new = _i32(context_lens), _i32(new_lens)
+    if ctx.ndim != 1 or new.shape != ctx.shape or ctx.numel() == 0:
+        raise ValueError("context_lens and new_lens must be vectors of the same batch")
+    batch = ctx.numel()
+    if block_table.ndim != 2 or block_table.shape[0] != batch or block_table.shape[1] == 0:
+        raise ValueError("block_table must be [batch, max_blocks]")
+    _exact_tensor(block_table, "block_table", torch.int32, block_table.shape)
+    free, head = _i32(free_pages), _i32(free_head)
+    if free.ndim != 1 or head.numel() != 1:
+        raise ValueError("free_pages must be a vector and free_head one number")
+    total_new = int(total_new)
+    if total_new < 0:
+        raise ValueError("total_new must not be negative")
+    # The five int32 results share one allocation.
+    ints = torch.empty(3 * batch + 3, dtype=torch.int32, device=dev)
+    seq, cu_q, cu_blocks, head_out = ints.split([batch, batch + 1, batch + 1, 1])
+    slots, positions = torch.empty(2, total_new, dtype=torch.int64, device=dev).unbind(0)
+    _call(dev, "ls_plan_pages", ctx.data_ptr(), new.data_ptr(), batch, block_table.data_ptr(),
+          block_table.shape[1], _ptr(free) if free.numel() else None, free.numel(),
+          head.data_ptr(), total_new, seq.data_ptr(), cu_q.data_ptr(), cu_blocks.data_ptr(),
+          _ptr(slots) if total_new else None, _ptr(positions) if total_new else None,
+          head_out.data_ptr(), status_word(dev).data_ptr(), _stream(dev))
+    return PagePlan(ctx, seq, cu_q, cu_blocks, slots, positions, head_out)
+
+
+def _check_cache(k_pages, v_pages, k_scale, v_scale):
+    """The cache's tensors, used in place: ``[num_pages, G, 64, 128]`` e4m3, ``[num_pages, G]``."""
+    if k_pages.ndim != 4 or k_pages.shape[2] != _native.LS_PAGE_TOKENS:
+        raise ValueError("k_pages must be [num_pages, num_kv_heads, 64, head_dim]")
+    _exact_tensor(k_pages, "k_pages", torch.float8_e4m3fn, k_pages.shape)
+    _exact_tensor(v_pages, "v_pages", torch.float8_e4m3fn, k_pages.shape)
+    _exact_tensor(k_scale, "k_scale", torch.float32, k_pages.shape[:2])
+    _exact_tensor(v_scale, "v_scale", torch.float32, k_pages.shape[:2])
+    return k_pages.shape[0], k_pages.shape[1], k_pages.shape[3]
+
+
+def _token_rows(t: torch.Tensor) -> torch.Tensor:
+    """bf16 ``[N, G, D]`` whose heads are contiguous and tokens 16-byte aligned (a
+    view into a fused projection passes as it is)."""
+    if t.dtype != torch.bfloat16:
+        t = t.to(torch.bfloat16)
+    if (t.stride(2) == 1 and t.stride(1) == t.shape[2] and t.stride(0) % 8 == 0
+            and t.stride(0) >= t.shape[1] * t.shape[2] and t.data_ptr() % 16 == 0):
+        return t
+    return t.contiguous()
+
+
+def append_kv(k: torch.Tensor, v: torch.Tensor, plan: PagePlan, k_pages: torch.Tensor,
+              v_pages: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor) -> None:
+    """Round a step's ``k``, ``v`` ``[total_new, G, 128]`` into the 8-bit cache (``ls_append_kv``).
+
+    ``k_pages``/``v_pages [num_pages, G, 64, 128]`` (e4m3) and
+    ``k_scale``/``v_scale [num_pages, G]`` (fp32, powers of two) are updated in
+    place.  A (page, head) scale covers the page's largest value and only
+    grows while the page fills; older codes are rescaled with it.
+    """
+    dev = _require_cuda(k, v, plan.context_lens, plan.seq_lens, plan.cu_seqlens_q, plan.cu_blocks,
+                        plan.slots, k_pages, v_pages, k_scale, v_scale)
+    num_pages, G, D = _check_cache(k_pages, v_pages, k_scale, v_scale)
+    if k.ndim != 3 or tuple(k.shape[1:]) != (G, D) or v.shape != k.shape:
+        raise ValueError("k and v must be [total_new, num_kv_heads, head_dim] of the cache")
+    n, batch = k.shape[0], plan.context_lens.numel()
+    _exact_tensor(plan.context_lens, "plan.context_lens", torch.int32, (batch,))
+    _exact_tensor(plan.seq_lens, "plan.seq_lens", torch.int32, (batch,))
+    _exact_tensor(plan.cu_seqlens_q, "plan.cu_seqlens_q", torch.int32, (batch + 1,))
+    _exact_tensor(plan.cu_blocks, "plan.cu_blocks", torch.int32, (batch + 1,))
+    _exact_tensor(plan.slots, "plan.slots", torch.int64, (n,))
+    if n == 0:
+        return
+    kb, vb = _token_rows(k), _token_rows(v)
+    _call(dev, "ls_append_kv", kb.data_ptr(), vb.data_ptr(), kb.stride(0), vb.stride(0), n, batch,
+          G, D, plan.context_lens.data_ptr(), plan.seq_lens.data_ptr(),
+          plan.cu_seqlens_q.data_ptr(), plan.cu_blocks.data_ptr(), plan.slots.data_ptr(),
+          k_pages.data_ptr(), v_pages.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
+          num_pages, status_word(dev).data_ptr(), _stream(dev))
+
+
+def paged_attn(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+               k_scale: torch.Tensor, v_scale: torch.Tensor, block_table: torch.Tensor,
+               seq_lens: torch.Tensor, cu_seqlens_q: torch.Tensor, max_seqlen_q: int,
+               max_seqlen_k: int, *, topk_idx: torch.Tensor | None = None,
+               softmax_scale: float | None = None, causal: bool = True,
+               return_lse: bool = False, out: torch.Tensor | None = None):
+    """Attention over the 8-bit paged cache (``ls_paged_attn``).
+
+    The counterpart of :func:`sparse_attn` for decode steps, drafts of a few
+    tokens and page-listed chunks: query row ``i`` of request ``b`` stands at
+    position ``seq_lens[b] - nq + i`` (its own keys are already cached).
+    ``topk_idx [G, total_q, T]`` lists each row's pages as the selection writes
+    them; ``None`` attends to every page.  Rows behind the last request are left
+    as they were in ``out``.
+    """
+    dev = _require_cuda(q, k_pages, v_pages, k_scale, v_scale, block_table, seq_lens,
+                        cu_seqlens_q, topk_idx)
+    num_pages, G, D = _check_cache(k_pages, v_pages, k_scale, v_scale)
+    if q.ndim != 3 or q.shape[2] != D or q.shape[1] % G:
+        raise ValueError("q must be [total_q, num_heads, head_dim], num_heads a multiple of the "
+                         "cache's heads")
+    qb = _bf16(q)
+    total_q, H, _ = qb.shape
+    table, seq, cu_q = _i32(block_table), _i32(seq_lens), _i32(cu_seqlens_q)
+    batch = seq.numel()
+    if seq.ndim != 1 or cu_q.shape != (batch + 1,) or table.ndim != 2 or table.shape[0] != batch:
+        raise ValueError("block_table [B, max_blocks], seq_lens [B] and cu_seqlens_q [B+1] must "
+                         "agree on the batch")
+    topk, idx = 0, None
+    if topk_idx is not None:
+        idx = _i32(topk_idx)
+        if idx.ndim != 3 or idx.shape[0] != G or idx.shape[1] != total_q or idx.shape[2] == 0:
+            raise ValueError("topk_idx must be [num_kv_heads, total_q, T] with T > 0")
+        topk = idx.shape[2]
+    direct = out if out is not None and q.dtype == torch.bfloat16 else None
+    if out is not None:
+        _exact_tensor(out, "out", q.dtype, q.shape)
+        if out.device != dev:
+            raise ValueError("all tensors must be on the same CUDA device")
+    if direct is None:
+        direct = torch.empty(total_q, H, D, dtype=torch.bfloat16, device=dev)
+        if out is not None:
+            direct.copy_(out)  # rows behind the last request keep their values
+    lse = torch.empty(H, total_q, dtype=torch.float32, device=dev) if return_lse else None
+    scale = float(softmax_scale) if softmax_scale is not None else 1.0 / math.sqrt(D)
+    nbytes = _native.load().ls_paged_attn_workspace_bytes()
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    _call(dev, "ls_paged_attn", qb.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
+          k_scale.data_ptr(), v_scale.data_ptr(), num_pages, table.data_ptr(), table.shape[1],
+          seq.data_ptr(), cu_q.data_ptr(), batch, int(max_seqlen_q), int(max_seqlen_k), total_q, H,
+          G, D, _ptr(idx), topk, scale, 1 if causal else 0, ws.data_ptr(), nbytes,
+          direct.data_ptr(), _ptr(lse), status_word(dev).data_ptr(), _stream(dev))
+    if out is None:
+        out = direct if q.dtype == torch.bfloat16 else direct.to(q.dtype)
+    elif direct is not out:
+        out.copy_(direct)
+    return (out, lse) if return_lse else out

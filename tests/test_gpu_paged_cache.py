@@ -1,0 +1,552 @@
+"""The 8-bit paged cache on the GPU against its 64-bit oracle (needs a B200).
+
+Tolerances:
+* planning: whole numbers, equal;
+* cache write: codes and scales equal bit for bit (both round the exact
+  quotient once, scales are powers of two);
+* attention, per output value, with A = sum w|v| and R = max sum |q||k| scale
+  of the row from the oracle and N its keys:
+    2^-8 (|ref| + e)  rounding of the bf16 output: half a step of the value
+  that is rounded, which is ref with an error of up to e, plus
+    e = A (2^-11 + 2 d + N 2^-24) + 2^-31 B  with d = 128 2^-23 R + 2^-20 and
+  B = max (w vs) sum |code|:
+  the weights are rounded to f16 (half a step 2^-11), a score of 128 products
+  is off by at most d (each fp32 addition 2^-23 relative when it truncates;
+  2^-20 for the exponential and the logarithms of the scales) which moves a
+  weight and the row sum by d each, and N fp32 additions of products.
+  Weights times value scale are held in f16 relative to a reference that puts
+  the largest at 2^6 or more, so a weight in f16's subnormals is off by up to
+  2^-25, which is 2^-31 of the largest.
+  Queries are held to 2^-25 of their row's largest value: 128 2^-25 is inside d.
+* log-sum-exp: d + N 2^-24 for the sum, and 2^-22 (|ref| + 64) for the
+  roundings of the reference exponent.
+"""
+import math
+
+import pytest
+import torch
+
+from oracle import paged_cache as ora
+
+pytestmark = pytest.mark.gpu
+
+if not torch.cuda.is_available():  # pragma: no cover - collected on CPU too
+    pytest.skip("needs CUDA", allow_module_level=True)
+
+from leanselect_b200 import _native, ops  # noqa: E402
+
+DEV = torch.device("cuda", 0)
+PAGE = 64
+FP8 = torch.float8_e4m3fn
+
+
+@pytest.fixture(autouse=True)
+def clean_status():
+    torch.cuda.synchronize()
+    ops.status_word(DEV).zero_()
+    yield
+    torch.cuda.synchronize()
+    assert ops.check_status(DEV) == 0
+
+
+def i32(v):
+    return torch.tensor(v, dtype=torch.int32, device=DEV)
+
+
+def prefix(v):
+    return [sum(v[:i]) for i in range(len(v) + 1)]
+
+
+def up(n):
+    return -(-n // PAGE)
+
+
+def tolerance(ref, bounds, n_keys):
+    mass, reach, grain = bounds
+    d = 128 * 2.0 ** -23 * reach[..., None] + 2.0 ** -20
+    e = mass * (2.0 ** -11 + 2 * d + n_keys * 2.0 ** -24) + 2.0 ** -31 * grain
+    return 2.0 ** -8 * (ref.abs() + e) + e
+
+
+# ---------------------------------------------------------------------------
+# plan_pages
+# ---------------------------------------------------------------------------
+
+def first_table(context, width, pool, gen):
+    """A block table for the cached tokens and the free list that is left."""
+    perm = torch.randperm(pool, generator=gen).tolist()
+    table = []
+    for c in context:
+        table.append([perm.pop() for _ in range(up(c))] + [-1] * (width - up(c)))
+    return table, perm
+
+
+@pytest.mark.parametrize("context, new, pad", [
+    ([0], [1], 0),
+    ([63], [1], 0),
+    ([64], [1], 0),
+    ([0, 5, 64, 127, 128], [0, 0, 0, 0, 0], 3),
+    ([0, 1, 63, 64, 65, 200], [1, 64, 1, 0, 63, 129], 0),
+    ([130, 0, 7], [3, 0, 300], 11),
+    ([0, 0, 640], [1000, 0, 1], 0),
+])
+def test_plan_small(context, new, pad):
+    gen = torch.Generator().manual_seed(1)
+    width = max(up(c + n) for c, n in zip(context, new)) + 2
+    table, free = first_table(context, width, 100, gen)
+    total = sum(new) + pad
+    dev_table = i32(table)
+    p = ops.plan_pages(i32(context), i32(new), dev_table, i32(free), i32([2]), total)
+    ref = ora.plan(context, new, table, free, 2, total)
+    check_plan(p, ref, dev_table, table)
+
+
+def check_plan(p, ref, dev_table, table):
+    assert dev_table.tolist() == table
+    assert p.seq_lens.tolist() == ref["seq"]
+    assert p.cu_seqlens_q.tolist() == ref["cu_q"]
+    assert p.cu_blocks.tolist() == ref["cu_blocks"]
+    assert p.slots.tolist() == ref["slots"]
+    assert p.positions.tolist() == ref["positions"]
+    assert p.free_head.tolist() == [ref["head"]]
+
+
+@pytest.mark.parametrize("batch, longest", [(1, 40000), (37, 3000), (700, 70), (3001, 3)])
+def test_plan_large_and_ragged(batch, longest):
+    gen = torch.Generator().manual_seed(batch)
+    context = torch.randint(0, 300, (batch,), generator=gen).tolist()
+    new = torch.randint(0, longest + 1, (batch,), generator=gen).tolist()
+    need = sum(up(c) + up(n) + 1 for c, n in zip(context, new))
+    width = max(up(c + n) for c, n in zip(context, new))
+    table, free = first_table(context, width, need, gen)
+    dev_table = i32(table)
+    p = ops.plan_pages(i32(context), i32(new), dev_table, i32(free), i32([0]), sum(new))
+    check_plan(p, ora.plan(context, new, table, free, 0, sum(new)), dev_table, table)
+
+
+def test_plan_at_its_largest_batch():
+    batch = _native.LS_MAX_PLAN_BATCH
+    context, new = [63] * batch, [2] * batch
+    table = [[i, -1] for i in range(batch)]
+    free = list(range(batch, 2 * batch))
+    dev_table = i32(table)
+    p = ops.plan_pages(i32(context), i32(new), dev_table, i32(free), i32([0]), 2 * batch)
+    check_plan(p, ora.plan(context, new, table, free, 0, 2 * batch), dev_table, table)
+
+
+def test_plan_out_of_pages_marks_tokens_and_status():
+    table = [[-1] * 4, [-1] * 4]
+    dev_table = i32(table)
+    p = ops.plan_pages(i32([0, 0]), i32([100, 70]), dev_table, i32([5, 6, 7]), i32([0]), 170)
+    check_plan(p, ora.plan([0, 0], [100, 70], table, [5, 6, 7], 0, 170), dev_table, table)
+    with pytest.raises(_native.LeanSelectError, match="PAGES"):
+        ops.check_status(DEV)
+
+
+@pytest.mark.parametrize("context, new, total", [
+    ([-1, 4], [2, 2], 4),      # a negative length counts as 0
+    ([0, 4], [-3, 2], 2),
+    ([0, 250], [1, 20], 21),   # past max_blocks = 4
+    ([0, 0], [5, 5], 7),       # more tokens than the packed rows
+])
+def test_plan_bad_lengths_are_reported(context, new, total):
+    dev_table = i32([[0, 1, 2, 3], [4, 5, 6, 7]])
+    p = ops.plan_pages(i32(context), i32(new), dev_table, i32([8, 9]), i32([0]), total)
+    slots = p.slots.tolist()
+    assert len(slots) == total and all(-1 <= s < 10 * 64 for s in slots)
+    if context[1] == 250:
+        assert slots[1 + 6:] == [-1] * 14 and slots[1] == 7 * 64 + 58
+    with pytest.raises(_native.LeanSelectError, match="SEQLENS"):
+        ops.check_status(DEV)
+
+
+def test_plan_refusals():
+    good = dict(context_lens=i32([0]), new_lens=i32([1]), block_table=i32([[-1]]),
+                free_pages=i32([0]), free_head=i32([0]), total_new=1)
+    for change in (dict(new_lens=i32([1, 1])), dict(block_table=i32([[-1], [-1]])),
+                   dict(block_table=i32([[-1]]).long()), dict(total_new=-1),
+                   dict(free_head=i32([0, 0])),
+                   dict(block_table=i32([[-1] * 4])[:, ::2])):
+        with pytest.raises(ValueError):
+            ops.plan_pages(**{**good, **change})
+
+
+# ---------------------------------------------------------------------------
+# append_kv
+# ---------------------------------------------------------------------------
+
+def empty_cache(pages, G, seed):
+    """Pages full of leftovers: any code but NaN, any scale."""
+    gen = torch.Generator().manual_seed(seed)
+    codes = [torch.randint(0, 127, (pages, G, PAGE, 128), generator=gen, dtype=torch.uint8)
+             for _ in range(2)]
+    scales = [torch.exp2(torch.randint(-8, 3, (pages, G), generator=gen).float())
+              for _ in range(2)]
+    return [c.view(FP8).to(DEV) for c in codes] + [s.to(DEV) for s in scales]
+
+
+def as_values(codes):
+    return codes.float().double().cpu()
+
+
+def run_append(context, new, G, k, v, cache, table):
+    width = len(table[0])
+    plan = ops.PagePlan(
+        i32(context), i32([c + n for c, n in zip(context, new)]), i32(prefix(new)),
+        i32(prefix([up(c + n) - c // PAGE if n else 0 for c, n in zip(context, new)])),
+        torch.tensor([table[b][p // PAGE] * PAGE + p % PAGE if table[b][p // PAGE] >= 0 else -1
+                      for b in range(len(new)) for p in range(context[b], context[b] + new[b])],
+                     dtype=torch.int64, device=DEV), None)
+    assert width
+    want = [as_values(cache[0]), as_values(cache[1]), cache[2].double().cpu(),
+            cache[3].double().cpu()]
+    ops.append_kv(k, v, plan, cache[0], cache[1], cache[2], cache[3])
+    ora.append(k.cpu(), context, new, table, want[0], want[2])
+    ora.append(v.cpu(), context, new, table, want[1], want[3])
+    for got, ref in zip((as_values(cache[0]), as_values(cache[1]), cache[2].double().cpu(),
+                         cache[3].double().cpu()), want):
+        assert torch.equal(got.nan_to_num(1234.0), ref.nan_to_num(1234.0))
+
+
+@pytest.mark.parametrize("context, new, G", [
+    ([0], [1], 1),
+    ([63], [1], 2),
+    ([64], [1], 2),
+    ([1], [63], 3),
+    ([0, 17, 64, 100], [64, 47, 0, 1], 2),
+    ([30, 0, 127, 5], [200, 65, 2, 700], 4),
+    ([3], [1], 16),
+])
+def test_append(context, new, G):
+    gen = torch.Generator().manual_seed(7)
+    width = max(up(c + n) for c, n in zip(context, new))
+    table, _ = first_table([c + n for c, n in zip(context, new)], width, 64, gen)
+    cache = empty_cache(64, G, 3)
+    n = sum(new)
+    # Magnitudes over many binades, so that scales grow, stay and hit old pages.
+    size = torch.exp2(torch.randint(-20, 12, (n, G, 1), generator=gen).float())
+    k = (torch.randn(n, G, 128, generator=gen) * size).bfloat16().to(DEV)
+    v = (torch.randn(n, G, 128, generator=gen)).bfloat16().to(DEV)
+    run_append(context, new, G, k, v, cache, table)
+
+
+def test_append_extremes():
+    """Zeros, subnormals, values at and next to 448 s, infinities and NaN."""
+    gen = torch.Generator().manual_seed(5)
+    rows = []
+    for special in (0.0, 1e-40, 448.0, 450.0, 2.0 ** -60, 3e38, math.inf, math.nan, 896.0):
+        r = torch.randn(64, 1, 128, generator=gen) * (1e-3 if special else 0.0)
+        if special in (1e-40, 2.0 ** -60):
+            r.zero_()
+        r[5, 0, 3] = special
+        r[9, 0, 4] = -special
+        rows.append(r)
+    k = torch.cat(rows).bfloat16().to(DEV)
+    cache = empty_cache(20, 1, 3)
+    table = [list(range(3, 3 + len(rows)))]
+    run_append([0], [k.shape[0]], 1, k, k.flip(0), cache, table)
+
+
+def test_append_grows_a_page_token_by_token():
+    """A page written one token at a time rescales what it holds, as the oracle does."""
+    gen = torch.Generator().manual_seed(11)
+    cache = empty_cache(4, 2, 9)
+    size = torch.exp2(torch.arange(70).float() / 6)[:, None, None]
+    k = (torch.randn(70, 2, 128, generator=gen) * size).bfloat16().to(DEV)
+    v = (torch.randn(70, 2, 128, generator=gen) / size).bfloat16().to(DEV)
+    for t in range(70):
+        run_append([t], [1], 2, k[t:t + 1], v[t:t + 1], cache, [[2, 0]])
+
+
+def test_append_views_of_a_fused_projection_and_other_types():
+    gen = torch.Generator().manual_seed(2)
+    qkv = torch.randn(90, 8 * 128, generator=gen).bfloat16().to(DEV)
+    k, v = qkv[:, 4 * 128:6 * 128].view(90, 2, 128), qkv[:, 6 * 128:].view(90, 2, 128)
+    assert not k.is_contiguous()
+    table = [[1, 3]]
+    run_append([20], [90], 2, k, v, empty_cache(5, 2, 1), table)
+    # Heads that are not contiguous, and fp32 values: rounded to bf16 on the way in.
+    odd = torch.randn(90, 128, 2, generator=gen).to(DEV).transpose(1, 2)
+    cache, twin = empty_cache(5, 2, 1), empty_cache(5, 2, 1)
+    for c, x in ((cache, odd), (twin, odd.bfloat16().contiguous())):
+        plan = ops.plan_pages(i32([0]), i32([90]), i32([[-1, -1]]), i32([4, 2]), i32([0]), 90)
+        ops.append_kv(x, x, plan, *c)
+    assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(cache, twin))
+
+
+def test_append_skips_tokens_without_pages_and_bad_pages():
+    gen = torch.Generator().manual_seed(2)
+    k = torch.randn(130, 1, 128, generator=gen).bfloat16().to(DEV)
+    run_append([0], [130], 1, k, k, empty_cache(6, 1, 1), [[4, -1, 2]])
+    cache = empty_cache(6, 1, 1)
+    before = [c.clone() for c in cache]
+    slots = torch.arange(6 * 64, 6 * 64 + 64, dtype=torch.int64, device=DEV)  # page 6 of 6
+    plan = ops.PagePlan(i32([0]), i32([64]), i32([0, 64]), i32([0, 1]), slots, None)
+    ops.append_kv(k[:64], k[:64], plan, *cache)
+    assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+               for a, b in zip(cache, before))
+    with pytest.raises(_native.LeanSelectError, match="PAGE_INDEX"):
+        ops.check_status(DEV)
+
+
+def test_append_refusals():
+    cache = empty_cache(3, 2, 1)
+    plan = ops.plan_pages(i32([0]), i32([5]), i32([[-1]]), i32([0]), i32([0]), 5)
+    k = torch.zeros(5, 2, 128, dtype=torch.bfloat16, device=DEV)
+    ops.append_kv(k, k, plan, *cache)
+    for args in ((k[:, :1], k[:, :1], plan, *cache), (k, k[:4], plan, *cache),
+                 (k[:4], k[:4], plan, *cache),
+                 (k, k, plan, cache[0].view(torch.uint8), *cache[1:]),
+                 (k, k, plan, cache[0], cache[1][:2], *cache[2:]),
+                 (k, k, plan, *cache[:2], cache[2].double(), cache[3])):
+        with pytest.raises(ValueError):
+            ops.append_kv(*args)
+
+
+# ---------------------------------------------------------------------------
+# paged_attn
+# ---------------------------------------------------------------------------
+
+def make_cache(seq, G, seed, sizes=(1.0, 1.0), nan_tail=True):
+    """Quantised random K/V of the requests in scattered pages; rows behind a
+    request's last token hold NaN codes."""
+    gen = torch.Generator().manual_seed(seed)
+    need = [up(max(n, 0)) for n in seq]
+    pool = sum(need) + 3
+    perm = torch.randperm(pool, generator=gen).tolist()
+    width = max(max(need), 1)
+    table = []
+    pools = []
+    for size in sizes:
+        x = torch.randn(pool, G, PAGE, 128, generator=gen, dtype=torch.float64) * size
+        x = x * torch.exp2(torch.randint(-3, 4, (pool, G, 1, 1), generator=gen).double())
+        amax = x.abs().amax((2, 3))
+        s = torch.exp2(torch.ceil(torch.log2(amax / 448.0)))
+        pools.append((ora.e4m3(x / s[:, :, None, None]), s.float()))
+    for n in need:
+        table.append([perm.pop() for _ in range(n)] + [-1] * (width - n))
+    codes = [c.float().to(FP8) for c, _ in pools]
+    if nan_tail:
+        for c in codes:
+            raw = c.view(torch.uint8)
+            for b, n in enumerate(seq):
+                if n > 0 and n % PAGE:
+                    raw[table[b][n // PAGE], :, n % PAGE:] = 0x7F
+            raw[perm] = 0x7F
+    return codes, [s for _, s in pools], table
+
+
+def run_attend(H, G, seq, nq, *, idx=None, causal=True, scale=None, seed=0, pad=0, sizes=(1.0, 1.0),
+               qsize=1.5, q_dtype=torch.bfloat16):
+    gen = torch.Generator().manual_seed(seed + 100)
+    codes, scales, table = make_cache(seq, G, seed, sizes)
+    N = sum(nq) + pad
+    q = (torch.randn(N, H, 128, generator=gen) * qsize).to(q_dtype)
+    cu = prefix(nq)
+    out = torch.full((N, H, 128), 3.0, dtype=q_dtype, device=DEV)
+    got, lse = ops.paged_attn(
+        q.to(DEV), codes[0].to(DEV), codes[1].to(DEV), scales[0].to(DEV), scales[1].to(DEV),
+        i32(table), i32(seq), i32(cu), max(nq), max(max(seq), 0), causal=causal,
+        topk_idx=None if idx is None else idx.to(DEV), softmax_scale=scale, return_lse=True,
+        out=out)
+    assert got.data_ptr() == out.data_ptr()
+    ref, ref_lse, bounds = ora.attend(
+        q.bfloat16(), codes[0].float(), codes[1].float(), scales[0], scales[1], table,
+        [max(n, 0) for n in seq], cu, idx, scale, causal, torch.full((N, H, 128), 3.0))
+    n_keys = max(max(seq), 1)
+    d = 128 * 2.0 ** -23 * bounds[1] + 2.0 ** -20
+    tol = tolerance(ref, bounds, n_keys)
+    err = (got.double().cpu() - ref).abs()
+    assert bool((err <= tol + 1e-30).all()), float((err - tol).max())
+    live = cu[-1]
+    a, r = lse.double().cpu()[:, :live], ref_lse[:, :live]
+    assert torch.equal(torch.isinf(a), torch.isinf(r))
+    fin = torch.isfinite(r)
+    ltol = d.T[:, :live] + n_keys * 2.0 ** -24 + 2.0 ** -22 * (r.abs() + 64)
+    assert bool(((a - r).abs()[fin] <= ltol[fin]).all()), float(((a - r).abs() - ltol)[fin].max())
+    return got
+
+
+@pytest.mark.parametrize("H, G", [(32, 2), (16, 2), (16, 1), (4, 4), (5, 1), (12, 6), (16, 16)])
+@pytest.mark.parametrize("length", [1, 16, 63, 64, 65, 1000])
+def test_decode_lengths_and_heads(H, G, length):
+    run_attend(H, G, [length], [1], seed=length)
+
+
+@pytest.mark.parametrize("causal", [True, False])
+def test_dense_ragged_batch(causal):
+    run_attend(32, 2, [1, 500, 64, 129, 2048, 77, 300], [1, 4, 0, 3, 1, 2, 70], causal=causal)
+
+
+def test_rows_without_keys_are_zero():
+    """Empty requests, and rows that stand before position 0."""
+    run_attend(16, 2, [0, 5, 0, 3], [1, 1, 2, 6])
+
+
+def test_rows_behind_the_last_request_are_left():
+    run_attend(16, 2, [200, 90], [2, 1], pad=5)
+
+
+@pytest.mark.parametrize("batch, length", [(1, 20000), (3, 7001), (150, 130), (400, 40)])
+def test_many_splits_and_many_rows(batch, length):
+    """One row cut into a part per CTA; several rows per CTA."""
+    gen = torch.Generator().manual_seed(batch)
+    seq = torch.randint(1, length + 1, (batch,), generator=gen).tolist()
+    seq[0] = length
+    run_attend(16, 1, seq, [1] * batch, seed=batch)
+
+
+@pytest.mark.parametrize("sizes, qsize", [((8.0, 1e-3), 1.5), ((0.01, 100.0), 4.0),
+                                          ((1.0, 2.0 ** -28), 1.5), ((1.0, 2.0 ** 44), 1.5),
+                                          ((2.0 ** -28, 1.0), 2.0 ** 28)])
+def test_scales_and_peaked_rows(sizes, qsize):
+    run_attend(32, 2, [700, 100], [2, 1], sizes=sizes, qsize=qsize, seed=4)
+
+
+def test_pages_of_very_different_value_scales():
+    """A row whose weight sits in a page of tiny values next to pages of large ones."""
+    gen = torch.Generator().manual_seed(6)
+    codes, scales, table = make_cache([256], 1, 6)
+    scales[1][table[0][0]] = 2.0 ** -30
+    scales[1][table[0][1]] = 2.0 ** 10
+    q = torch.randn(1, 16, 128, generator=gen).bfloat16()
+    # the first page's first key points along the query
+    codes[0][table[0][0], 0, 0] = (q[0, 0].float() * 100).clamp(-448, 448).to(FP8)
+    scales[0][table[0][0]] = 0.25
+    ref, _, bounds = ora.attend(q, codes[0].float(), codes[1].float(), scales[0], scales[1],
+                                     table, [256], [0, 1])
+    got = ops.paged_attn(q.to(DEV), codes[0].to(DEV), codes[1].to(DEV), scales[0].to(DEV),
+                         scales[1].to(DEV), i32(table), i32([256]), i32([0, 1]), 1, 256)
+    tol = tolerance(ref, bounds, 256)
+    assert bool(((got.double().cpu() - ref).abs() <= tol).all())
+
+
+def page_lists(seq, nq, G, T, seed, kind):
+    gen = torch.Generator().manual_seed(seed)
+    rows = []
+    for b, n in enumerate(nq):
+        for i in range(n):
+            last = max(0, (seq[b] - n + i) // PAGE)
+            per = []
+            for _ in range(G):
+                if kind == "empty" and (i + b) % 2 == 0:
+                    per.append([-1] * T)
+                    continue
+                pick = torch.randperm(last + 1, generator=gen)[:T].tolist()
+                if kind == "ascending":
+                    pick = sorted(pick)
+                elif kind == "repeats":
+                    pick = (pick + pick[:3] + [-1, 0, 0])[:T]
+                elif kind == "future":     # pages past the row's position, within the request
+                    pick = torch.randperm(up(max(seq[b], 1)), generator=gen)[:T].tolist()
+                per.append(pick + [-1] * (T - len(pick)))
+            rows.append(per)
+    return torch.tensor(rows, dtype=torch.int32).transpose(0, 1).contiguous()
+
+
+@pytest.mark.parametrize("kind", ["ascending", "shuffled", "repeats", "future", "empty"])
+@pytest.mark.parametrize("H, G, T", [(32, 2, 67), (16, 2, 128), (6, 2, 5), (16, 1, 1)])
+def test_listed_pages(kind, H, G, T):
+    seq, nq = [3000, 64, 1, 900], [1, 2, 1, 17]
+    run_attend(H, G, seq, nq, idx=page_lists(seq, nq, G, T, 5, kind), seed=T)
+
+
+def test_listed_chunk_many_rows():
+    seq, nq = [2000], [333]
+    run_attend(16, 2, seq, nq, idx=page_lists(seq, nq, 2, 12, 5, "ascending"), seed=2)
+
+
+def test_listed_rows_with_padding_and_no_causal_limit():
+    seq, nq = [700, 300], [3, 2]
+    idx = page_lists(seq, nq, 2, 7, 5, "future")
+    idx = torch.nn.functional.pad(idx, (0, 0, 0, 4), value=0)
+    run_attend(32, 2, seq, nq, idx=idx, pad=4, causal=False)
+
+
+def test_bad_pages_are_passed_over_and_reported():
+    codes, scales, table = make_cache([300, 64], 2, 3)
+    table[0][1] = 10 ** 6
+    table[0][3] = -1
+    gen = torch.Generator().manual_seed(3)
+    q = torch.randn(2, 32, 128, generator=gen).bfloat16()
+    args = (codes[0].to(DEV), codes[1].to(DEV), scales[0].to(DEV), scales[1].to(DEV), i32(table),
+            i32([300, 64]), i32([0, 1, 2]), 1, 300)
+    for idx in (None, torch.tensor([[[3, 1, 0, 4], [0, 9, -1, -1]]] * 2, dtype=torch.int32)):
+        got = ops.paged_attn(q.to(DEV), *args, topk_idx=None if idx is None else idx.to(DEV))
+        ref, _, bounds = ora.attend(q, codes[0].float(), codes[1].float(), scales[0], scales[1],
+                                     table, [300, 64], [0, 1, 2], idx)
+        assert bool(((got.double().cpu() - ref).abs() <= tolerance(ref, bounds, 300)).all())
+        with pytest.raises(_native.LeanSelectError, match="PAGE_INDEX"):
+            ops.check_status(DEV)
+
+
+def test_bad_lengths_are_reported_and_stay_in_bounds():
+    codes, scales, table = make_cache([100, 64], 1, 3)
+    cache = (codes[0].to(DEV), codes[1].to(DEV), scales[0].to(DEV), scales[1].to(DEV), i32(table))
+    q = torch.randn(3, 16, 128, device=DEV).bfloat16()
+    for seq, cu in (([100, 100000], [0, 1, 2]), ([-5, 64], [0, 1, 2]), ([100, 64], [0, 2, 9]),
+                    ([100, 64], [0, 3, 1])):
+        ops.paged_attn(q, *cache, i32(seq), i32(cu), 1, 128)
+        with pytest.raises(_native.LeanSelectError):
+            ops.check_status(DEV)
+
+
+def test_equal_calls_give_equal_bits_and_other_types_are_cast():
+    a = run_attend(32, 2, [5000, 3], [1, 1], seed=9)
+    b = run_attend(32, 2, [5000, 3], [1, 1], seed=9)
+    assert torch.equal(a, b)
+    run_attend(32, 2, [130], [2], seed=9, pad=2, q_dtype=torch.float32)
+
+
+def test_attention_refusals():
+    codes, scales, table = make_cache([100], 2, 3)
+    q = torch.zeros(1, 32, 128, dtype=torch.bfloat16, device=DEV)
+    good = [q, codes[0].to(DEV), codes[1].to(DEV), scales[0].to(DEV), scales[1].to(DEV),
+            i32(table), i32([100]), i32([0, 1]), 1, 100]
+    ops.paged_attn(*good)
+    for at, value in ((0, q[:, :31]), (0, q[..., :64]), (1, good[1].view(torch.uint8)),
+                      (2, good[2][:1]), (3, good[3].double()), (5, i32(table + table)),
+                      (6, i32([100, 100])), (7, i32([0]))):
+        with pytest.raises(ValueError):
+            ops.paged_attn(*[value if i == at else x for i, x in enumerate(good)])
+    with pytest.raises(ValueError):
+        ops.paged_attn(*good, topk_idx=i32([[[0]]]))
+    with pytest.raises(ValueError):
+        ops.paged_attn(*good, out=q.float())
+    with pytest.raises(_native.LeanSelectError, match="heads per group"):
+        ops.paged_attn(torch.zeros(1, 34, 128, dtype=torch.bfloat16, device=DEV), *good[1:])
+
+
+# ---------------------------------------------------------------------------
+# a run of the three, as a decode loop uses them
+# ---------------------------------------------------------------------------
+
+def test_prompt_then_decode_steps():
+    """Two requests: ragged prompts, then steps of one token, against the oracle
+    over what the cache holds."""
+    gen = torch.Generator().manual_seed(21)
+    G, H, width, pool = 2, 32, 8, 24
+    cache = empty_cache(pool, G, 5)
+    table, free = [[-1] * width for _ in range(3)], torch.randperm(pool, generator=gen).tolist()
+    dev_table, dev_free, head = i32(table), i32(free), i32([0])
+    context, at = [0, 0, 0], 0
+    ctx = i32(context)
+    mirror = [as_values(cache[0]), as_values(cache[1]), cache[2].double().cpu(),
+              cache[3].double().cpu()]
+    for new in ([130, 0, 63], [1, 1, 1], [1, 1, 1], [0, 70, 1], [2, 1, 1]):
+        n = sum(new)
+        plan = ops.plan_pages(ctx, i32(new), dev_table, dev_free, head, n)
+        ref = ora.plan(context, new, table, free, at, n)
+        check_plan(plan, ref, dev_table, table)
+        k, v = (torch.randn(n, G, 128, generator=gen).bfloat16() for _ in range(2))
+        q = torch.randn(n, H, 128, generator=gen).bfloat16()
+        ops.append_kv(k.to(DEV), v.to(DEV), plan, *cache)
+        ora.append(k, context, new, table, mirror[0], mirror[2])
+        ora.append(v, context, new, table, mirror[1], mirror[3])
+        got = ops.paged_attn(q.to(DEV), *cache, dev_table, plan.seq_lens, plan.cu_seqlens_q,
+                             max(new), max(ref["seq"]))
+        want, _, bounds = ora.attend(q, *mirror, table, ref["seq"], ref["cu_q"])
+        tol = tolerance(want, bounds, 256)
+        assert bool(((got.double().cpu() - want).abs() <= tol).all())
+        context, at = ref["seq"], ref["head"]
+        ctx, head = plan.seq_lens, plan.free_head

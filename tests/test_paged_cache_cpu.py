@@ -1,0 +1,144 @@
+"""The paged cache's argument checks and its 64-bit oracle, without a GPU."""
+import ctypes
+
+import pytest
+import torch
+
+from leanselect_b200 import _native, ops
+from oracle import paged_cache as ora
+
+FAKE = ctypes.c_void_p(1 << 20)  # never dereferenced: validation fails first
+ODD = ctypes.c_void_p((1 << 20) + 4)
+INVALID, UNSUPPORTED, ALIGNMENT = (_native.LS_ERR_INVALID_ARGUMENT, _native.LS_ERR_UNSUPPORTED,
+                                   _native.LS_ERR_ALIGNMENT)
+
+
+def refused(name, base, changes, code, text):
+    args = list(base)
+    for at, value in changes.items():
+        args[at] = value
+    lib = _native.load()
+    assert getattr(lib, name)(*args) == code
+    assert text in lib.ls_last_error()
+
+
+PLAN = [FAKE, FAKE, 4, FAKE, 8, FAKE, 16, FAKE, 100, FAKE, FAKE, FAKE, FAKE, FAKE, ODD, None, None]
+
+
+@pytest.mark.parametrize("changes, code, text", [
+    ({0: None}, INVALID, b"null"),
+    ({9: None}, INVALID, b"null output"),
+    ({14: FAKE}, INVALID, b"free_head"),
+    ({2: 0}, INVALID, b"sizes"),
+    ({4: 0}, INVALID, b"sizes"),
+    ({5: None}, INVALID, b"free_pages"),
+    ({8: -1}, INVALID, b"total_new"),
+    ({8: 1 << 31}, INVALID, b"total_new"),
+    ({12: None}, INVALID, b"slots"),
+    ({2: _native.LS_MAX_PLAN_BATCH + 1}, UNSUPPORTED, b"LS_MAX_PLAN_BATCH"),
+])
+def test_plan_refusals(changes, code, text):
+    refused("ls_plan_pages", PLAN, changes, code, text)
+
+
+APPEND = [FAKE, FAKE, 256, 256, 10, 2, 2, 128, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE,
+          FAKE, 5, None, None]
+
+
+@pytest.mark.parametrize("changes, code, text", [
+    ({0: None}, INVALID, b"null"),
+    ({13: None}, INVALID, b"null cache"),
+    ({17: 0}, INVALID, b"cache sizes"),
+    ({17: 1 << 24}, INVALID, b"out of range"),
+    ({7: 64}, UNSUPPORTED, b"head_dim"),
+    ({2: 128}, INVALID, b"strides"),
+    ({3: 260}, ALIGNMENT, b"strides"),
+    ({1: ODD}, ALIGNMENT, b"v is not"),
+    ({14: ODD}, ALIGNMENT, b"v_pages"),
+    ({5: 0}, INVALID, b"sizes"),
+])
+def test_append_refusals(changes, code, text):
+    refused("ls_append_kv", APPEND, changes, code, text)
+
+
+def test_append_of_nothing_is_ok():
+    args = list(APPEND)
+    args[0] = args[1] = args[12] = None
+    args[4] = 0
+    assert _native.load().ls_append_kv(*args) == _native.LS_OK
+
+
+ATTEND = [FAKE, FAKE, FAKE, FAKE, FAKE, 5, FAKE, 4, FAKE, FAKE, 2, 1, 200, 2, 32, 2, 128, FAKE, 7,
+          0.0, 1, FAKE, 1 << 30, FAKE, None, None, None]
+
+
+@pytest.mark.parametrize("changes, code, text", [
+    ({0: None}, INVALID, b"null"),
+    ({1: None}, INVALID, b"null cache"),
+    ({6: None}, INVALID, b"null"),
+    ({16: 64}, UNSUPPORTED, b"head_dim"),
+    ({14: 34}, UNSUPPORTED, b"heads per group"),
+    ({14: 31}, INVALID, b"multiple"),
+    ({18: 129}, UNSUPPORTED, b"LS_MAX_TOPK"),
+    ({17: None}, INVALID, b"topk_idx"),
+    ({7: 0}, INVALID, b"sizes"),
+    ({12: -1}, INVALID, b"max_seqlen"),
+    ({0: ODD}, ALIGNMENT, b"q is not"),
+    ({22: 100}, INVALID, b"workspace"),
+    ({21: None}, INVALID, b"workspace"),
+    ({21: ODD}, ALIGNMENT, b"workspace"),
+    ({13: 1 << 31}, INVALID, b"out of range"),
+])
+def test_attention_refusals(changes, code, text):
+    refused("ls_paged_attn", ATTEND, changes, code, text)
+
+
+def test_attention_of_no_rows_is_ok():
+    args = list(ATTEND)
+    args[13] = 0
+    assert _native.load().ls_paged_attn(*args) == _native.LS_OK
+
+
+def test_cpu_tensors_raise():
+    i32 = torch.zeros(2, dtype=torch.int32)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        ops.plan_pages(i32, i32, torch.zeros(2, 4, dtype=torch.int32), i32, i32[:1], 0)
+    pages = torch.zeros(1, 2, 64, 128).to(torch.float8_e4m3fn)
+    scale = torch.ones(1, 2)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        ops.paged_attn(torch.zeros(2, 32, 128), pages, pages, scale, scale,
+                       torch.zeros(2, 1, dtype=torch.int32), i32, torch.zeros(3, dtype=torch.int32),
+                       1, 1)
+
+
+def test_oracle_rounding_is_that_of_torch():
+    """Every representable value, every midpoint between two and its neighbours."""
+    codes = torch.arange(127, dtype=torch.uint8).view(torch.float8_e4m3fn).double()
+    mid = (codes[1:] + codes[:-1]) / 2
+    x = torch.cat([codes, mid, mid * (1 + 2.0 ** -20), mid * (1 - 2.0 ** -20), -mid])
+    assert torch.equal(ora.e4m3(x), x.float().to(torch.float8_e4m3fn).double())
+    assert float(ora.e4m3(torch.tensor(1e30, dtype=torch.float64))) == 448.0
+    assert ora.e4m3(torch.tensor(float("nan"), dtype=torch.float64)).isnan()
+
+
+def test_oracle_plan_by_hand():
+    table = [[7, -1, -1], [5, 6, -1]]
+    p = ora.plan([63, 128], [3, 1], table, [9, 8], 0, 6)
+    assert table == [[7, 9, -1], [5, 6, 8]]
+    assert p["slots"] == [7 * 64 + 63, 9 * 64, 9 * 64 + 1, 8 * 64, -1, -1]
+    assert p["positions"] == [63, 64, 65, 128, 0, 0]
+    assert (p["seq"], p["cu_q"], p["cu_blocks"], p["head"]) == ([66, 129], [0, 3, 4], [0, 2, 3], 2)
+
+
+def test_oracle_attention_is_softmax_over_the_listed_keys():
+    torch.manual_seed(0)
+    k, v = (ora.e4m3(torch.randn(4, 1, 64, 128, dtype=torch.float64)) for _ in range(2))
+    q = torch.randn(1, 2, 128)
+    one = torch.ones(4, 1)
+    out, lse, _ = ora.attend(q, k, v, one, one, [[2, 0, 3]], [130], [0, 1],
+                                idx=torch.tensor([[[2, 0, 2, -1]]]))
+    kk = torch.cat([k[2, 0], k[3, 0, :2]])
+    vv = torch.cat([v[2, 0], v[3, 0, :2]])
+    ref = torch.nn.functional.scaled_dot_product_attention(q[0].double(), kk, vv)
+    assert torch.allclose(out[0], ref, atol=1e-12)
+    assert torch.allclose(lse[:, 0], torch.logsumexp(q[0].double() @ kk.T / 128 ** 0.5, -1))
