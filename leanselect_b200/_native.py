@@ -6,6 +6,8 @@ operation raises.  Build it with ``python -m leanselect_b200.build``.
 from __future__ import annotations
 
 import ctypes
+import importlib.machinery
+import importlib.util
 import os
 import threading
 from pathlib import Path
@@ -85,6 +87,7 @@ SIZE_FUNCS = {"ls_select_pages_workspace_bytes": [_I64, _I32, _I32],
 
 _lock = threading.Lock()
 _lib = None
+_fast = None
 
 
 class LeanSelectError(RuntimeError):
@@ -126,14 +129,39 @@ def load(path: os.PathLike | str | None = None) -> ctypes.CDLL:
         return lib
 
 
-def call(name: str, *args) -> None:
-    """Invoke a C-ABI entry point and raise :class:`LeanSelectError` on failure."""
-    lib = load()
-    rc = getattr(lib, name)(*args)
+def binding():
+    """The compiled Python entry of the paged-cache operators (``csrc/binding.cpp``)."""
+    global _fast
+    if _fast is None:
+        load()  # the library it links against, with its error message when missing
+        with _lock:
+            if _fast is None:
+                import torch  # noqa: F401  (the module links against its libraries)
+
+                target = LIB_PATH.with_name("_binding.so")
+                if not target.exists():
+                    raise RuntimeError(f"leanselect_b200 binding not found at {target}; build it "
+                                       "with `python -m leanselect_b200.build`")
+                loader = importlib.machinery.ExtensionFileLoader("_binding", str(target))
+                spec = importlib.util.spec_from_file_location("_binding", target, loader=loader)
+                module = importlib.util.module_from_spec(spec)
+                loader.exec_module(module)
+                _fast = module
+    return _fast
+
+
+def raise_for(name: str, rc: int) -> None:
+    """Raise :class:`LeanSelectError` for a C-ABI return code other than ``LS_OK``."""
     if rc != LS_OK:
+        lib = load()
         text = lib.ls_status_string(rc).decode()
         detail = lib.ls_last_error().decode()
         raise LeanSelectError(rc, f"{name} failed with {text}: {detail}")
+
+
+def call(name: str, *args) -> None:
+    """Invoke a C-ABI entry point and raise :class:`LeanSelectError` on failure."""
+    raise_for(name, getattr(load(), name)(*args))
 
 
 def version() -> str:

@@ -21,6 +21,11 @@ ROOT = PKG.parent
 CSRC = PKG / "csrc"
 LIB_DIR = PKG / "_lib"
 LIB = LIB_DIR / "libleanselect_b200.so"
+# The compiled Python entry of the paged-cache operators; it is built against
+# the installed torch, whose version its stamp file records.
+BINDING = LIB_DIR / "_binding.so"
+BINDING_STAMP = LIB_DIR / "_binding.torch"
+BINDING_SOURCE = CSRC / "binding.cpp"
 SOURCES = ["prep.cu", "score_select.cu", "sparse_attn.cu", "capi.cu", "backbone.cu", "noalloc.cu",
            "waitprobe.cu", "select_f32.cu", "paged_cache.cu", "paged_attn.cu"]
 HEADERS = ["common.cuh", "launch.h", "topk_rows.cuh", "page_list.cuh"]
@@ -46,10 +51,52 @@ def _stale() -> bool:
     return any(p.stat().st_mtime > built for p in inputs)
 
 
+def _binding_stale(torch_version: str) -> bool:
+    if not BINDING.exists() or not BINDING_STAMP.exists():
+        return True
+    if BINDING_STAMP.read_text() != torch_version:
+        return True
+    built = BINDING.stat().st_mtime
+    inputs = [BINDING_SOURCE, ROOT / "include" / "leanselect_b200.h", Path(__file__)]
+    return any(p.stat().st_mtime > built for p in inputs)
+
+
+def build_binding(force: bool = False, verbose: bool = False) -> Path:
+    """Compile the Python entry module against the installed torch (host code only)."""
+    import sysconfig
+
+    import torch
+
+    if not force and not _binding_stale(torch.__version__):
+        return BINDING
+    home = Path(torch.__file__).resolve().parent
+    cuda = Path(nvcc()).resolve().parents[1]
+    tmp = BINDING.with_suffix(".so.tmp")
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           "-isystem", str(home / "include"),
+           "-isystem", str(home / "include" / "torch" / "csrc" / "api" / "include"),
+           "-isystem", sysconfig.get_paths()["include"], "-isystem", str(cuda / "include"),
+           str(BINDING_SOURCE), "-o", str(tmp), f"-L{LIB_DIR}", f"-L{home / 'lib'}",
+           "-lleanselect_b200", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python",
+           "-Wl,-rpath,$ORIGIN"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    subprocess.run(cmd, check=True)
+    os.replace(tmp, BINDING)
+    BINDING_STAMP.write_text(torch.__version__)
+    return BINDING
+
+
 def build(force: bool = False, verbose: bool = False, extra_flags=()) -> Path:
-    """Compile every kernel for sm_100a and link the shared library."""
-    if not force and not _stale():
-        return LIB
+    """Compile every kernel for sm_100a, link the shared library and its Python entry."""
+    if force or _stale():
+        _build_library(verbose, extra_flags)
+    build_binding(force, verbose)
+    return LIB
+
+
+def _build_library(verbose: bool, extra_flags) -> None:
     LIB_DIR.mkdir(exist_ok=True)
     obj_dir = LIB_DIR / "obj"
     obj_dir.mkdir(exist_ok=True)
@@ -70,7 +117,6 @@ def build(force: bool = False, verbose: bool = False, extra_flags=()) -> Path:
         print(" ".join(cmd), flush=True)
     subprocess.run(cmd, check=True)
     os.replace(tmp, LIB)
-    return LIB
 
 
 def main(argv=None) -> int:

@@ -601,6 +601,13 @@ def plan_pages(context_lens: torch.Tensor, new_lens: torch.Tensor, block_table: 
     the last request get slot -1).  The next step passes ``plan.seq_lens`` and
     ``plan.free_head`` on; nothing here reads the device back.
     """
+    if context_lens.is_cuda:
+        got = _native.binding().plan_pages(context_lens, new_lens, block_table, free_pages,
+                                           free_head, int(total_new),
+                                           status_word(context_lens.device))
+        if got is not None:
+            _native.raise_for("ls_plan_pages", got[0])
+            return PagePlan(context_lens, *got[1:])
     dev = _require_cuda(context_lens, new_lens, block_table, free_pages, free_head)
     ctx, new = _i32(context_lens), _i32(new_lens)
     if ctx.ndim != 1 or new.shape != ctx.shape or ctx.numel() == 0:
@@ -658,6 +665,13 @@ def append_kv(k: torch.Tensor, v: torch.Tensor, plan: PagePlan, k_pages: torch.T
     place.  A (page, head) scale covers the page's largest value and only
     grows while the page fills; older codes are rescaled with it.
     """
+    if k.is_cuda:
+        rc = _native.binding().append_kv(k, v, plan.context_lens, plan.seq_lens,
+                                         plan.cu_seqlens_q, plan.cu_blocks, plan.slots, k_pages,
+                                         v_pages, k_scale, v_scale, status_word(k.device))
+        if rc is not None:
+            _native.raise_for("ls_append_kv", rc)
+            return
     dev = _require_cuda(k, v, plan.context_lens, plan.seq_lens, plan.cu_seqlens_q, plan.cu_blocks,
                         plan.slots, k_pages, v_pages, k_scale, v_scale)
     num_pages, G, D = _check_cache(k_pages, v_pages, k_scale, v_scale)
@@ -694,6 +708,14 @@ def paged_attn(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
     them; ``None`` attends to every page.  Rows behind the last request are left
     as they were in ``out``.
     """
+    if q.is_cuda:
+        got = _native.binding().paged_attn(
+            q, k_pages, v_pages, k_scale, v_scale, block_table, seq_lens, cu_seqlens_q,
+            int(max_seqlen_q), int(max_seqlen_k), topk_idx, softmax_scale or 0.0, bool(causal),
+            bool(return_lse), out, status_word(q.device))
+        if got is not None:
+            _native.raise_for("ls_paged_attn", got[0])
+            return got[1:] if return_lse else got[1]
     dev = _require_cuda(q, k_pages, v_pages, k_scale, v_scale, block_table, seq_lens,
                         cu_seqlens_q, topk_idx)
     num_pages, G, D = _check_cache(k_pages, v_pages, k_scale, v_scale)
@@ -723,7 +745,7 @@ def paged_attn(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
         if out is not None:
             direct.copy_(out)  # rows behind the last request keep their values
     lse = torch.empty(H, total_q, dtype=torch.float32, device=dev) if return_lse else None
-    scale = float(softmax_scale) if softmax_scale is not None else 1.0 / math.sqrt(D)
+    scale = float(softmax_scale or 0.0)  # 0 selects D^-0.5
     nbytes = _native.load().ls_paged_attn_workspace_bytes()
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     _call(dev, "ls_paged_attn", qb.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
