@@ -817,13 +817,13 @@ int ls_append_kv(const uint16_t* k, const uint16_t* v, int64_t k_stride, int64_t
 }
 
 namespace {
-// Bytes of one CTA's share of the paged attention workspace: the header, two
+// Bytes of one range's share of the paged attention workspace: the header, two
 // partial rows of 16 heads (128 sums, row reference and row sum).
 constexpr size_t kPagedPartFloats = 16 * (128 + 2);
-constexpr size_t kPagedCtaBytes = 16 + 2 * kPagedPartFloats * sizeof(float);
+constexpr size_t kPagedRangeBytes = 16 + 2 * kPagedPartFloats * sizeof(float);
 }  // namespace
 
-size_t ls_paged_attn_workspace_bytes(void) { return kPagedMaxCtas * kPagedCtaBytes; }
+size_t ls_paged_attn_workspace_bytes(void) { return kPagedMaxRanges * kPagedRangeBytes; }
 
 int ls_paged_attn(const uint16_t* q, const uint8_t* k_pages, const uint8_t* v_pages,
                   const float* k_scale, const float* v_scale, int64_t num_pages,
@@ -885,15 +885,18 @@ int ls_paged_attn(const uint16_t* q, const uint8_t* k_pages, const uint8_t* v_pa
   a.out = out;
   a.lse = lse;
   a.headers = static_cast<int2*>(workspace);
-  a.part_ml = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kPagedMaxCtas * 16);
-  a.part_o = a.part_ml + 2 * kPagedMaxCtas * 16 * 2;
+  a.part_ml = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kPagedMaxRanges * 16);
+  a.part_o = a.part_ml + 2 * kPagedMaxRanges * 16 * 2;
   a.status = status;
-  // At most one CTA per scheduled page: the caller's max_seqlen_k bounds the
-  // pages of a dense row (a longer request only gets fewer CTAs).
+  // At most one range per scheduled page: the caller's max_seqlen_k bounds the
+  // pages of a dense row (a longer request only gets fewer ranges).
+  LS_REQUIRE(total_q * num_kv_heads * std::max<int64_t>(topk > 0 ? topk : max_blocks, 1) <
+                 (int64_t{1} << 31),
+             "total_q * num_kv_heads * pages per row out of range");
   const int64_t per_row = topk > 0 ? topk : std::max<int64_t>(1, (int64_t{max_seqlen_k} + 63) / 64);
   const int64_t want = total_q * num_kv_heads * per_row;
-  const int ctas = static_cast<int>(std::min<int64_t>({want, 2 * sms, kPagedMaxCtas}));
-  err = launch_paged_attn(a, ctas, static_cast<cudaStream_t>(stream));
+  const int ranges = static_cast<int>(std::min<int64_t>({want, 2 * sms, kPagedMaxRanges}));
+  err = launch_paged_attn(a, ranges, static_cast<cudaStream_t>(stream));
   return err == cudaSuccess ? LS_OK : cuda_fail(err, "paged_attn launch");
 }
 

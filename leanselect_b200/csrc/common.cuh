@@ -74,6 +74,13 @@ __device__ __forceinline__ void mbar_arrive_expect_tx(uint64_t* bar, uint32_t by
                : "memory");
 }
 
+// Announces transaction bytes without arriving.
+__device__ __forceinline__ void mbar_expect_tx(uint64_t* bar, uint32_t bytes) {
+  asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)),
+               "r"(bytes)
+               : "memory");
+}
+
 __device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
   uint32_t ok = 0;
   asm volatile(
@@ -89,16 +96,20 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
 // Waits for phase `parity` of `bar` to complete.  Returns false (and records
 // LS_DEVERR_TIMEOUT) if it has not completed after `timeout_ns` of wall
 // time, or if another thread of the CTA already gave up (`abort_flag` set).
+// The clock is first read after 64 tries: reading it costs more than most
+// waits last.
 __device__ __forceinline__ bool mbar_wait_for(uint64_t* bar, uint32_t parity, int32_t* status,
                                               volatile int* abort_flag, uint64_t timeout_ns) {
   if (mbar_try_wait(bar, parity)) return true;
-  const uint64_t start = globaltimer();
+  uint64_t start = 0;
   uint32_t spins = 0;
   while (true) {
     if (mbar_try_wait(bar, parity)) return true;
     if ((++spins & 63u) == 0) {
       if (abort_flag != nullptr && *abort_flag) return false;
-      if (globaltimer() - start > timeout_ns) {
+      const uint64_t now = globaltimer();
+      if (start == 0) start = now;
+      if (now - start > timeout_ns) {
         report(status, LS_DEVERR_TIMEOUT);
         if (abort_flag != nullptr) *abort_flag = 1;
         return false;

@@ -172,7 +172,7 @@ struct AppendArgs {
 cudaError_t launch_append_kv(const AppendArgs& args, cudaStream_t stream);
 
 // Attention over the paged cache (paged_attn.cu).
-constexpr int kPagedMaxCtas = 2 * 148;  // two resident CTAs on each of the B200's SMs
+constexpr int kPagedMaxRanges = 2 * 148;  // work ranges: two on each of the B200's SMs
 
 struct PagedAttnArgs {
   CUtensorMap tm_k;       // K codes as [num_pages * G * 64, 128] bytes, box {128, 64}, 128B swizzle
@@ -196,13 +196,13 @@ struct PagedAttnArgs {
   float scale_log2;       // softmax_scale * log2(e)
   uint16_t* out;
   float* lse;
-  int2* headers;          // workspace: per CTA, the row it leaves unfinished and that row's last CTA
-  float* part_ml;         // [2 * CTAs, 16, 2]: row reference (log2) and row sum
-  float* part_o;          // [2 * CTAs, 16, 128]
+  int2* headers;          // workspace: per range, the row it leaves unfinished and that row's last range
+  float* part_ml;         // [2 * ranges, 16, 2]: row reference (log2) and row sum
+  float* part_o;          // [2 * ranges, 16, 128]
   int32_t* status;
 };
 
-cudaError_t launch_paged_attn(const PagedAttnArgs& args, int ctas, cudaStream_t stream);
+cudaError_t launch_paged_attn(const PagedAttnArgs& args, int ranges, cudaStream_t stream);
 
 // Host-side argument checks of ls_select_pages other than its workspace
 // (shared with ls_select_pages_noalloc); LS_OK or the LS_ERR_* code it sets.

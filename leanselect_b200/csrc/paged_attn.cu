@@ -24,6 +24,7 @@
 // paged_merge_kernel joins them.  The cut depends on the shapes and lengths
 // alone, and no sum uses atomics, so equal calls give equal bits.
 #include <cuda_fp16.h>
+#include <cuda_fp8.h>
 
 #include "common.cuh"
 #include "launch.h"
@@ -33,43 +34,66 @@ namespace ls {
 namespace {
 
 constexpr int kPage = LS_PAGE_TOKENS;
-constexpr int kStages = 4;
 constexpr int kTileBytes = kPage * 128;      // one page of one group, K or V
 constexpr int kStageBytes = 2 * kTileBytes;
-constexpr int kConsumers = 4;                // warps; each owns 16 keys of every page
-constexpr int kThreads = 32 * (kConsumers + 1);
+constexpr int kStages = 2;                   // ring of a warp pair
+constexpr int kTeams = 2;                    // teams per CTA, each with a range of its own
+constexpr int kWarps = 4;                    // consumer warps of a team: two pairs
+constexpr int kPairs = 2;                    // pairs take alternate pages, 32 keys a warp
+constexpr int kThreads = 128 * (kTeams + 1);
+constexpr int kProducerRegs = 72, kConsumerRegs = 216, kLaunchRegs = 168;
+static_assert(kProducerRegs + kTeams * kConsumerRegs <= (kTeams + 1) * kLaunchRegs,
+              "the split must fit the registers the block is launched with");
+static_assert(kTeams * kPairs == 4, "warpgroup 0 has one producer warp per pair");
+constexpr int kMinUnits = 2;                 // pages a range has at least
+constexpr int kRingBytes = kStages * kStageBytes;
+constexpr int kSumBytes = kWarps * 16 * 128 * 4;  // a team's row sums, one set per warp
 constexpr float kSlack = 14.f, kHeadroom = 6.f;  // binades, see above
 constexpr float kMinScale = 0x1p-40f, kMaxScale = 0x1p48f;
 
 enum StageFlag { kFirst = 1, kLast = 2, kData = 4, kStop = 8 };
 
-// What a consumer needs to know of one ring stage.
-struct StageMeta {
-  int flags;
+// What a pair's consumers need to know of one stage.
+struct __align__(16) PageDesc {
   int key0;        // position of the page's first key
   float k_scale, v_log2, v_inv;
   int limit;       // last visible position (-1: none)
-  int token, group;
-  int part;        // workspace part, -1: the row is whole in this CTA
+  int token;
+  int row;         // StageFlag | group << 4 | (workspace part + 1) << 20, part -1: none
+  int y;           // the page's first row in the tensor maps (-1: no data)
+};
+constexpr int kDescs = 64;  // a batch of 32 never reaches the stages still in the ring
+
+// The work unit a range begins at: unit `unit` of row (token, group), dense:
+// of request `b`, token being its row in the request.
+struct Start {
+  int b, group, token, unit;
+};
+
+struct PairSmem {
+  uint64_t full[kStages];
+  uint64_t empty[kStages];
+  PageDesc desc[kDescs];
+  int32_t pages[LS_MAX_TOPK];  // listed: the row's sorted pages
+};
+
+struct TeamSmem {
+  PairSmem pair[kPairs];
+  uint64_t join;   // the consumer warps' meeting point, bounded like every wait
+  int abort_flag;
+  Start start;     // where the team's range begins
+  float m_part[2][kWarps][16];  // alternate rows use alternate halves
+  float l_part[2][kWarps][16];
 };
 
 struct PagedSmem {
-  uint64_t full[kStages];
-  uint64_t empty[kStages];
-  uint64_t join;   // the consumer warps' meeting point, bounded like every wait
-  StageMeta meta[kStages];
-  int abort_flag;
-  int64_t scan[kConsumers + 1];
-  int32_t start_b;
-  int64_t start_off;
-  int32_t pages[LS_MAX_TOPK];
-  float m_part[kConsumers][16];
-  float l_part[kConsumers][16];
+  TeamSmem team[kTeams];
+  int scan[kThreads / 32];
 };
 
 __device__ __forceinline__ void mma_f16_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
                                               uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 "
       "{%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
@@ -111,8 +135,62 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
+// One page of one group, K then V, into a ring stage.
+__device__ __forceinline__ void load_page(const PagedAttnArgs& args, uint8_t* stage, uint64_t* bar,
+                                          int y) {
+  tma_load_2d(stage, &args.tm_k, bar, 0, y);
+  tma_load_2d(stage + kTileBytes, &args.tm_v, bar, 0, y);
+}
+
 __device__ __forceinline__ float bf16_lo(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float bf16_hi(uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); }
+
+// Query fragments of one row of heads in f16, scaled by a power of two so that
+// the row's largest value is near 1: f16 then holds every value to 2^-25 of
+// the largest.  The 32 dims a quad lane holds of a key row (32c ..) are the
+// contraction's order: k-step kk takes dims 32c + 4kk .. + 3.  kHalf: at most
+// 8 heads, rows 8 .. 15 of the tile stay zero.
+template <bool kHalf>
+__device__ __forceinline__ void load_query(const uint16_t* q, int gq, int heads, float scale_log2,
+                                           uint32_t (&qa)[8][4], float* f0, float* f1) {
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    const int h = gq + 8 * half;
+    if (kHalf && half == 1) {
+#pragma unroll
+      for (int kk = 0; kk < 8; ++kk) qa[kk][1] = qa[kk][3] = 0;
+      break;
+    }
+    const uint4* src = reinterpret_cast<const uint4*>(q + h * 128);
+    uint4 raw[4];
+    float amax = 0.f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) raw[k] = h < heads ? __ldg(src + k) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const uint32_t w[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        amax = fmaxf(amax, fmaxf(fabsf(bf16_lo(w[j])), fabsf(bf16_hi(w[j]))));
+    }
+    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+    // The exponent is kept to where the factor stays normal under every page
+    // scale.
+    const int e = min(max(static_cast<int>(__float_as_uint(amax) >> 23) - 127, -60), 78);
+    const float down = __int_as_float((127 - e) << 23);
+    const float factor = scale_log2 * __int_as_float((127 + e) << 23);
+    if (half == 0) *f0 = factor; else *f1 = factor;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const uint32_t w[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        qa[2 * k + (j >> 1)][half + 2 * (j & 1)] =
+            pack_f16x2(bf16_lo(w[j]) * down, bf16_hi(w[j]) * down);
+    }
+  }
+}
 
 // Byte offset of 16-byte chunk `chunk` (0..7) of row `row` in a 128B-swizzled box.
 __device__ __forceinline__ uint32_t sw128(int row, int chunk) {
@@ -121,183 +199,204 @@ __device__ __forceinline__ uint32_t sw128(int row, int chunk) {
 
 // Pages a request of `len` cached tokens is scheduled with: at least one, so
 // that every row is visited and written.
-__device__ __forceinline__ int64_t scheduled_pages(int64_t len) {
+__device__ __forceinline__ int scheduled_pages(int len) {
   return len > 0 ? (len + kPage - 1) / kPage : 1;
 }
 
 // A request as the kernels see it: lengths that would leave the packed rows
 // or the block table are cut and reported.
 struct Request {
-  int64_t q0;
-  int nq, len;
+  int q0, nq, len;
   bool bad;
 };
 
 __device__ __forceinline__ Request load_request(const PagedAttnArgs& a, int b) {
   Request r;
   r.q0 = __ldg(a.cu_q + b);
-  int64_t nq = __ldg(a.cu_q + b + 1) - r.q0;
-  int64_t len = __ldg(a.seq_lens + b);
-  const int64_t most = static_cast<int64_t>(a.max_blocks) * kPage;
-  r.bad = r.q0 < 0 || nq < 0 || r.q0 + nq > a.total_q || len < 0 || len > most;
-  if (r.q0 < 0 || nq < 0 || r.q0 + nq > a.total_q) nq = 0;
-  r.nq = static_cast<int>(nq);
-  r.len = static_cast<int>(min(max(len, int64_t{0}), most));
+  const int end = __ldg(a.cu_q + b + 1), len = __ldg(a.seq_lens + b);
+  const int most = a.max_blocks * kPage;  // at most 2^30
+  const bool rows_ok = r.q0 >= 0 && end >= r.q0 && end <= a.total_q;
+  r.bad = !rows_ok || len < 0 || len > most;
+  r.nq = rows_ok ? end - r.q0 : 0;
+  r.len = min(max(len, 0), most);
   return r;
 }
 
-// First work unit of CTA i when `work` units are cut into n ranges, and the
-// CTA that unit w belongs to.
-__device__ __forceinline__ int64_t range_start(int64_t i, int64_t work, int64_t n) {
-  return i * work / n;
-}
-__device__ __forceinline__ int range_of(int64_t w, int64_t work, int64_t n) {
-  return static_cast<int>(((w + 1) * n + work - 1) / work - 1);
-}
+// `work` units (pages) cut into ranges of at least kMinUnits, as equal as can
+// be; the caller's checks keep work below 2^31.
+struct Cut {
+  int ranges, size, longer;  // `longer` ranges have one unit more
+  __device__ __forceinline__ Cut(int work) {
+    ranges = min(static_cast<int>(gridDim.x) * kTeams, max(1, (work + kMinUnits - 1) / kMinUnits));
+    size = work / ranges;
+    longer = work - size * ranges;
+  }
+  __device__ __forceinline__ int start(int i) const { return i * size + min(i, longer); }
+};
 
-__global__ void __launch_bounds__(kThreads, 2) paged_attn_kernel(const __grid_constant__ PagedAttnArgs args) {
+template <bool kHalf>
+__global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_constant__ PagedAttnArgs args) {
   extern __shared__ __align__(16) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
-  uint8_t* stages = smem;
-  float* acc = reinterpret_cast<float*>(stages + kStages * kStageBytes);  // [warps][16][128]
-  PagedSmem* sm = reinterpret_cast<PagedSmem*>(acc + kConsumers * 16 * 128);
+  PagedSmem* shared =
+      reinterpret_cast<PagedSmem*>(smem + kTeams * (kPairs * kRingBytes + kSumBytes));
 
-  const int warp = threadIdx.x >> 5;
+  // The merge kernel may be set up from now on; it waits for this grid's end.
+  asm volatile("griddepcontrol.launch_dependents;");
+
+  const int warp_id = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   const int G = args.num_groups;
   const bool listed = args.topk > 0;
 
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < kStages; ++s) {
-      mbar_init(&sm->full[s], 1);
-      mbar_init(&sm->empty[s], kConsumers);
-    }
-    mbar_init(&sm->join, kConsumers);
-    sm->abort_flag = 0;
+  if (threadIdx.x < kTeams) {
+    TeamSmem* t = &shared->team[threadIdx.x];
+    for (int p = 0; p < kPairs; ++p)
+      for (int s = 0; s < kStages; ++s) {
+        mbar_init(&t->pair[p].full[s], 1);
+        mbar_init(&t->pair[p].empty[s], kWarps / kPairs);
+      }
+    mbar_init(&t->join, kWarps);
+    t->abort_flag = 0;
     fence_barrier_init();
   }
 
-  // ---- the work of all rows, and where this CTA's range starts
+  // ---- the work of all rows, and where the teams' ranges start
   // listed: row r = (group, token) has `topk` units, ordered group-major.
   // dense: request by request, (group, token) rows of scheduled_pages units.
-  int64_t work;
-  int64_t rows_listed = 0;
+  const int range0 = static_cast<int>(blockIdx.x) * kTeams;
+  int work, rows_listed = 0;
   if (listed) {
-    const int64_t rows = min(max(static_cast<int64_t>(__ldg(args.cu_q + args.batch)), int64_t{0}),
-                             args.total_q);
-    rows_listed = rows;
-    work = rows * G * args.topk;
-    __syncthreads();
+    rows_listed = min(max(__ldg(args.cu_q + args.batch), 0), static_cast<int>(args.total_q));
+    work = rows_listed * G * args.topk;
+    const Cut cut(work);
+    if (threadIdx.x < kTeams && range0 + static_cast<int>(threadIdx.x) < cut.ranges && work > 0) {
+      const int w0 = cut.start(range0 + threadIdx.x);
+      const int row = w0 / args.topk;
+      shared->team[threadIdx.x].start = {-1, row / rows_listed, row % rows_listed,
+                                         w0 - row * args.topk};
+    }
   } else {
     const int per = (args.batch + kThreads - 1) / kThreads;
     const int b0 = min(static_cast<int>(threadIdx.x) * per, args.batch);
     const int b1 = min(b0 + per, args.batch);
-    int64_t own = 0;
+    int own = 0;
     bool bad = false;
+    Request r{0, 0, 0, false};
+#pragma unroll 1
     for (int b = b0; b < b1; ++b) {
-      const Request r = load_request(args, b);
-      own += static_cast<int64_t>(r.nq) * G * scheduled_pages(r.len);
+      r = load_request(args, b);
+      own += r.nq * G * scheduled_pages(r.len);
       bad = bad || r.bad;
     }
     if (bad && blockIdx.x == 0) report(args.status, LS_DEVERR_SEQLENS);
-    int64_t x = own;
-#pragma unroll
+    int before = own;
+#pragma unroll 1
     for (int o = 1; o < 32; o <<= 1) {
-      const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
-      if (lane >= o) x += y;
+      const int y = __shfl_up_sync(0xffffffffu, before, o);
+      if (lane >= o) before += y;
     }
-    if (lane == 31) sm->scan[warp] = x;
+    if (lane == 31) shared->scan[warp_id] = before;
+    before -= own;
     __syncthreads();
-    int64_t before = x - own;
     work = 0;
-    for (int w = 0; w < kConsumers + 1; ++w) {
-      if (w < warp) before += sm->scan[w];
-      work += sm->scan[w];
+#pragma unroll 1
+    for (int w = 0; w < kThreads / 32; ++w) {
+      const int x = shared->scan[w];
+      if (w < warp_id) before += x;
+      work += x;
     }
-    const int64_t n_all = min(static_cast<int64_t>(gridDim.x), work);
-    const int64_t w0 = blockIdx.x < n_all ? range_start(blockIdx.x, work, n_all) : -1;
-    if (w0 >= before && w0 < before + own) {
-      int64_t at = before;
+    const Cut cut(work);
+#pragma unroll 1
+    for (int t = 0; t < kTeams; ++t) {
+      int off = range0 + t < cut.ranges ? cut.start(range0 + t) - before : -1;
+      if (off < 0 || off >= own) continue;
       for (int b = b0; b < b1; ++b) {
-        const Request r = load_request(args, b);
-        const int64_t units = static_cast<int64_t>(r.nq) * G * scheduled_pages(r.len);
-        if (w0 < at + units) {
-          sm->start_b = b;
-          sm->start_off = w0 - at;
+        if (b1 - b0 > 1) r = load_request(args, b);
+        const int pages = scheduled_pages(r.len), units = r.nq * G * pages;
+        if (off < units) {
+          const int row = off / pages;
+          shared->team[t].start = {b, row / r.nq, row % r.nq, off - row * pages};
           break;
         }
-        at += units;
+        off -= units;
       }
     }
-    __syncthreads();
   }
-  const int64_t n_ctas = min(static_cast<int64_t>(gridDim.x), work);
-  int2* header = args.headers + blockIdx.x;
-  if (blockIdx.x >= n_ctas) {
-    if (threadIdx.x == 0) *header = make_int2(-1, 0);
-    return;
-  }
-  const int64_t w_begin = range_start(blockIdx.x, work, n_ctas);
-  const int64_t w_end = range_start(blockIdx.x + 1, work, n_ctas);
+  __syncthreads();
+
+  // From here on the warpgroups part for good: the producers give registers
+  // up, the consumers take them (each before anything else in its branch).
+  const bool producer = warp_id < 4;
+  const int team = producer ? warp_id / kPairs : (warp_id >> 2) - 1;
+  const int pair = producer ? warp_id % kPairs : (warp_id & 3) / (kWarps / kPairs);
+  TeamSmem* sm = &shared->team[team];
+  PairSmem* ps = &sm->pair[pair];
+  uint8_t* ring = smem + (team * kPairs + pair) * kRingBytes;
+  float* sums = reinterpret_cast<float*>(smem + kTeams * kPairs * kRingBytes + team * kSumBytes);
+  const Cut cut(work);
+  const int range = range0 + team;
+  const bool idle = range >= cut.ranges || work == 0;
   volatile int* abort_flag = &sm->abort_flag;
 
-  if (warp == kConsumers) {
+  if (producer) {
     // ------------------------------------------------------------- producer
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kProducerRegs));
+    int2* header = args.headers + range;
+    if (idle) {
+      if (pair == 0 && lane == 0) *header = make_int2(-1, 1);
+      return;
+    }
+    int left = cut.start(range + 1) - cut.start(range);
     if (lane == 0) {
       tma_prefetch_desc(&args.tm_k);
       tma_prefetch_desc(&args.tm_v);
     }
-    int fill = 0;   // stages filled so far
-    bool ok = true;
-    int2 head = make_int2(-1, 0);
-    int64_t w = w_begin;
-    int b = listed ? 0 : sm->start_b;
-    int64_t off = listed ? 0 : sm->start_off;  // dense: unit inside request b
-    while (w < w_end && ok) {
-      // ---- the row that unit w belongs to
-      int64_t units, a, token;
-      int g;
-      Request req;
+    int fill = 0, slot = 0;  // stages filled so far, and the ring slot of the next
+    uint32_t phase = 1;      // parity that says the slot is free
+    bool ok = true;          // lane 0's view; the warp learns of it per batch
+    int2 head = make_int2(-1, 1);
+    Start at = sm->start;
+    Request req{0, 0, 0, false};
+    if (!listed) req = load_request(args, at.b);
+    while (left > 0 && ok) {
+      // ---- the row that the next unit belongs to
+      int token;
       if (listed) {
-        units = args.topk;
-        const int64_t row = w / units;
-        a = w % units;
-        g = static_cast<int>(row / rows_listed);
-        token = row % rows_listed;
-        b = find_sequence(args.cu_q, args.batch, token);
-        req = load_request(args, b);
-        if (req.bad && lane == 0) report(args.status, LS_DEVERR_SEQLENS);
-      } else {
-        if (b >= args.batch) break;  // lengths changed under the kernel
-        req = load_request(args, b);
-        units = scheduled_pages(req.len);
-        if (off >= units * req.nq * G) {
-          off = 0;
-          ++b;
-          continue;
+        token = at.token;
+        if (at.b < 0 || token < req.q0 || token >= req.q0 + req.nq) {
+          at.b = find_sequence(args.cu_q, args.batch, token);
+          req = load_request(args, at.b);
+          if (req.bad && lane == 0) report(args.status, LS_DEVERR_SEQLENS);
         }
-        const int64_t row = off / units;
-        a = off % units;
-        g = static_cast<int>(row / req.nq);
-        token = req.q0 + row % req.nq;
+      } else {
+        token = req.q0 + at.token;
       }
-      const int64_t e = min(units, a + (w_end - w));
-      const int t_rel = static_cast<int>(token - req.q0);
+      const int units = listed ? args.topk : scheduled_pages(req.len);
+      const int unit_end = min(units, at.unit + left);
+      const int t_rel = token - req.q0;
       int limit = req.len - 1;
       if (args.causal) limit = min(limit, req.len - req.nq + t_rel);
       if (t_rel < 0 || t_rel >= req.nq) limit = -1;
-      const int whole = a == 0 && e == units;
-      const int part = whole ? -1 : 2 * static_cast<int>(blockIdx.x) + (a == 0 ? 1 : 0);
-      if (a == 0 && e < units)
-        head = make_int2(static_cast<int>(token * G + g),
-                         range_of(w - a + units - 1, work, n_ctas));
+      const int g = at.group;
+      // A row cut by the range's borders goes to the workspace: its begin to
+      // the range's second part, what continues an earlier range to the first.
+      int part = -1;
+      if (at.unit > 0) {
+        part = 2 * range;
+        if (unit_end < units) head.y = 0;  // and goes on behind this range too
+      } else if (unit_end < units) {
+        part = 2 * range + 1;
+        head.x = token * G + g;
+      }
 
-      // ---- its pages, and this CTA's share of them
+      // ---- its pages, and this pair's share of them: every other one, or
+      // one stage without data
       int n_row;
       if (listed) {
-        const int32_t* list = args.topk_idx + (static_cast<int64_t>(g) * args.total_q + token) *
-                                                  args.topk;
+        const int32_t* list =
+            args.topk_idx + (static_cast<int64_t>(g) * args.total_q + token) * args.topk;
         const int n_pages = (req.len + kPage - 1) / kPage;
         int32_t v[4];
         bool bad = false;
@@ -306,128 +405,157 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attn_kernel(const __grid_co
           const int pos = 32 * r + lane;
           const int32_t p = pos < args.topk ? __ldg(list + pos) : -1;
           bad = bad || p >= n_pages;
-          v[r] = (p >= 0 && p < n_pages && static_cast<int64_t>(p) * kPage <= limit) ? p
-                                                                                  : kPageSentinel;
+          v[r] = (p >= 0 && p < n_pages && p * kPage <= limit) ? p : kPageSentinel;
         }
-        if (__any_sync(0xffffffffu, bad) && lane == 0) report(args.status, LS_DEVERR_PAGE_INDEX);
+        if (bad) report(args.status, LS_DEVERR_PAGE_INDEX);
         __syncwarp();
-        n_row = warp_compact_pages(v, sm->pages, lane);
+        n_row = warp_compact_pages(v, ps->pages, lane);
         __syncwarp();
       } else {
         n_row = limit >= 0 ? limit / kPage + 1 : 0;
       }
-      const int lo = static_cast<int>(a * n_row / units), hi = static_cast<int>(e * n_row / units);
+      const int lo = min(at.unit, n_row) + pair, hi = min(unit_end, n_row);
+      const int count = max(0, (hi - lo + 1) >> 1);
+      const int n_stages = max(1, count);
 
-      const int32_t* table = args.block_table + static_cast<int64_t>(b) * args.max_blocks;
-      bool first = true;
-      for (int base = lo; base < hi && ok; base += 32) {
-        // 32 pages' table entries and scales at once, one per lane.
-        const int i = base + lane;
-        int32_t logical = -1, page = -1;
-        float ks = 0.f, vs = 1.f;
-        if (i < hi) {
-          logical = listed ? sm->pages[i] : i;
-          page = __ldg(table + logical);
-          if (page < 0 || page >= args.num_pages) {
-            page = -1;
-            report(args.status, LS_DEVERR_PAGE_INDEX);
+      const int32_t* table = args.block_table + static_cast<int64_t>(at.b) * args.max_blocks;
+      for (int base = 0; base < n_stages && ok; base += 32) {
+        // 32 pages at once, one per lane: table entry, then both scales.
+        PageDesc d;
+        d.y = -1;
+        d.key0 = 0;
+        float ks = 1.f, vs = 1.f;
+        if (base + lane < count) {
+          const int i = lo + 2 * (base + lane);
+          const int logical = listed ? ps->pages[i] : i;
+          const int page = __ldg(table + logical);
+          d.key0 = logical * kPage;
+          if (page >= 0 && page < args.num_pages) {
+            d.y = (page * G + g) * kPage;
+            ks = __ldg(args.k_scale + static_cast<int64_t>(page) * G + g);
+            vs = __ldg(args.v_scale + static_cast<int64_t>(page) * G + g);
           } else {
-            const int64_t at = static_cast<int64_t>(page) * G + g;
-            ks = __ldg(args.k_scale + at);
-            vs = __ldg(args.v_scale + at);
+            report(args.status, LS_DEVERR_PAGE_INDEX);
+          }
+        }
+        const int n = min(32, n_stages - base);
+        // The first copies start before the scales are here.
+        const int early = min(n, kStages);
+        int y0[kStages];
+#pragma unroll
+        for (int j = 0; j < kStages; ++j) y0[j] = __shfl_sync(0xffffffffu, d.y, j);
+        int s0 = slot;
+        uint32_t p0 = phase;
+        if (lane == 0) {
+#pragma unroll
+          for (int j = 0; j < kStages; ++j) {
+            if (j < early && ok) {
+              ok = mbar_wait(&ps->empty[s0], p0, args.status, abort_flag);
+              if (ok && y0[j] >= 0) {
+                mbar_expect_tx(&ps->full[s0], kStageBytes);
+                load_page(args, ring + s0 * kStageBytes, &ps->full[s0], y0[j]);
+              }
+              if (++s0 == kStages) {
+                s0 = 0;
+                p0 ^= 1;
+              }
+            }
           }
         }
         ks = fminf(fmaxf(ks, kMinScale), kMaxScale);
         vs = fminf(fmaxf(vs, kMinScale), kMaxScale);
-        const float v_log2 = __log2f(vs), v_inv = 1.f / vs;
-        const int n = min(32, hi - base);
-        for (int j = 0; j < n; ++j) {
-          const int32_t lp = __shfl_sync(0xffffffffu, logical, j);
-          const int32_t pp = __shfl_sync(0xffffffffu, page, j);
-          const float kj = __shfl_sync(0xffffffffu, ks, j);
-          const float lj = __shfl_sync(0xffffffffu, v_log2, j);
-          const float ij = __shfl_sync(0xffffffffu, v_inv, j);
-          const bool last = base + j + 1 == hi;
-          if (pp < 0 && !last && !first) continue;
-          const int s = fill % kStages;
-          if (lane == 0) {
-            ok = mbar_wait(&sm->empty[s], ((fill / kStages) & 1) ^ 1, args.status, abort_flag);
-            if (ok) {
-              StageMeta m;
-              m.flags = (first ? kFirst : 0) | (last ? kLast : 0) | (pp >= 0 ? kData : 0);
-              m.key0 = lp * kPage;
-              m.k_scale = kj;
-              m.v_log2 = lj;
-              m.v_inv = ij;
-              m.limit = limit;
-              m.token = static_cast<int>(token);
-              m.group = g;
-              m.part = part;
-              sm->meta[s] = m;
-              if (pp >= 0) {
-                uint8_t* st = stages + s * kStageBytes;
-                const int32_t y = (pp * G + g) * kPage;
-                mbar_arrive_expect_tx(&sm->full[s], kStageBytes);
-                tma_load_2d(st, &args.tm_k, &sm->full[s], 0, y);
-                tma_load_2d(st + kTileBytes, &args.tm_v, &sm->full[s], 0, y);
+        d.k_scale = ks;
+        d.v_log2 = __log2f(vs);
+        d.v_inv = 1.f / vs;
+        d.limit = limit;
+        d.token = token;
+        const int nth = base + lane;
+        d.row = (nth == 0 ? kFirst : 0) | (nth + 1 == n_stages ? kLast : 0) |
+                (d.y >= 0 ? kData : 0) | g << 4 | (part + 1) << 20;
+        if (lane < n) ps->desc[(fill + lane) % kDescs] = d;
+        __syncwarp();
+        if (lane == 0) {
+          for (int j = 0; j < n; ++j) {
+            if (j < early) {
+              // also after a wait that gave up: what is in flight may land
+              mbar_arrive(&ps->full[slot]);
+            } else {
+              ok = ok && mbar_wait(&ps->empty[slot], phase, args.status, abort_flag);
+              if (!ok) break;
+              const int y = ps->desc[(fill + j) % kDescs].y;
+              if (y >= 0) {
+                mbar_arrive_expect_tx(&ps->full[slot], kStageBytes);
+                load_page(args, ring + slot * kStageBytes, &ps->full[slot], y);
               } else {
-                mbar_arrive(&sm->full[s]);
+                mbar_arrive(&ps->full[slot]);
               }
             }
-          }
-          ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
-          if (!ok) break;
-          ++fill;
-          first = false;
-        }
-      }
-      if (ok && lo >= hi) {
-        // A share without pages still writes its row (or its empty part).
-        const int s = fill % kStages;
-        if (lane == 0) {
-          ok = mbar_wait(&sm->empty[s], ((fill / kStages) & 1) ^ 1, args.status, abort_flag);
-          if (ok) {
-            StageMeta m{};
-            m.flags = kFirst | kLast;
-            m.limit = limit;
-            m.token = static_cast<int>(token);
-            m.group = g;
-            m.part = part;
-            sm->meta[s] = m;
-            mbar_arrive(&sm->full[s]);
+            if (++slot == kStages) {
+              slot = 0;
+              phase ^= 1;
+            }
           }
         }
         ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
-        if (ok) ++fill;
+        fill += n;
       }
-      off += e - a;
-      w += e - a;
+      // ---- on to the next row
+      left -= unit_end - at.unit;
+      at.unit = 0;
+      if (listed) {
+        if (++at.token == rows_listed) {
+          at.token = 0;
+          ++at.group;
+        }
+      } else if (++at.token >= req.nq) {
+        at.token = 0;
+        if (++at.group == G) {
+          at.group = 0;
+          do {
+            ++at.b;
+            if (at.b >= args.batch) left = 0;  // lengths changed under the kernel
+            else req = load_request(args, at.b);
+          } while (left > 0 && req.nq == 0);
+        }
+      }
     }
     if (lane == 0) {
-      const int s = fill % kStages;
-      if (ok) ok = mbar_wait(&sm->empty[s], ((fill / kStages) & 1) ^ 1, args.status, abort_flag);
+      if (ok) ok = mbar_wait(&ps->empty[slot], phase, args.status, abort_flag);
       if (ok) {
-        sm->meta[s].flags = kStop;
-        mbar_arrive(&sm->full[s]);
+        ps->desc[fill % kDescs].row = kStop;
+        mbar_arrive(&ps->full[slot]);
+      } else {
+        // Copies in flight must land before the CTA gives up its memory: the
+        // last kStages slots filled, newest first.
+        for (int k = 0; k < kStages; ++k) {
+          if (slot == 0) {
+            slot = kStages;
+            phase ^= 1;
+          }
+          --slot;
+          mbar_wait(&ps->full[slot], phase ^ 1, nullptr, nullptr);
+        }
       }
-      *header = ok ? head : make_int2(-1, 0);
-      if (!ok) {
-        // Copies in flight must land before the CTA gives up its memory.
-        for (int k = max(0, fill - kStages); k < fill; ++k)
-          mbar_wait(&sm->full[k % kStages], (k / kStages) & 1, nullptr, nullptr);
-      }
+      if (pair == 0) *header = ok ? head : make_int2(-1, 1);
     }
     return;
   }
 
   // -------------------------------------------------------------- consumers
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kConsumerRegs));
+  if (idle) return;
   const int gq = lane >> 2, c = lane & 3;  // fragment row / key, and quad lane
   const int Hg = args.heads_per_group;
+  const int warp = warp_id & 3;
+  const int key_base = (warp & 1) * 32;
+  // Lane offsets inside a stage.  K: chunk 2c of key gq of a tile (the next
+  // chunk is 16 bytes off, before or behind); V: chunk gq of keys 2c, 2c + 1.
+  const uint32_t k_off = sw128(gq, 2 * c) + key_base * 128;
+  const uint32_t v_off0 = sw128(2 * c, gq) + key_base * 128 + kTileBytes;
+  const uint32_t v_off1 = sw128(2 * c + 1, gq) + key_base * 128 + kTileBytes;
   uint32_t qa[8][4];
   float o[16][4];
   float f0 = 0.f, f1 = 0.f;                 // score factors of rows gq and gq + 8
-  float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
-  const int key_base = warp * 16;
   uint32_t joins = 0;
   // All consumer warps meet; false once a wait has given up anywhere (the
   // row then stays unwritten).
@@ -437,234 +565,214 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attn_kernel(const __grid_co
     return mbar_wait(&sm->join, joins++ & 1, args.status, abort_flag);
   };
 
-  for (int i = 0;; ++i) {
-    const int s = i % kStages;
-    if (!mbar_wait(&sm->full[s], (i / kStages) & 1, args.status, abort_flag)) return;
-    const StageMeta meta = sm->meta[s];
-    if (meta.flags & kStop) return;
+  int slot = 0, stage = 0, row_parity = 0;
+  uint32_t phase = 0;
+  // The first row is known from the start: its queries load while its pages do.
+  int token = sm->start.token, group = sm->start.group;
+  if (!listed) token += __ldg(args.cu_q + sm->start.b);
+  while (true) {
+    load_query<kHalf>(
+        args.q + (static_cast<int64_t>(token) * args.num_heads + group * Hg) * 128 + 32 * c, gq, Hg,
+        args.scale_log2, qa, &f0, &f1);
+#pragma unroll
+    for (int j = 0; j < 16; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
+    float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+    int flags;
+    do {
+      if (!mbar_wait(&ps->full[slot], phase, args.status, abort_flag)) return;
+      const PageDesc& desc = ps->desc[stage++ % kDescs];
+      flags = desc.row;
 
-    if (meta.flags & kFirst) {
-      // Q fragments.  The 32 dims a quad lane holds of a key row (32c ..) are
-      // the contraction's order: k-step kk takes dims 32c + 4kk .. + 3.
+      // Keys of this warp that the row may see: all 32, some or none.
+      const int seen = desc.limit - (desc.key0 + key_base) + 1;
+      if ((flags & kData) && seen > 0) {
+        const uint32_t st = smem_u32(ring + slot * kStageBytes);
+        // ---- S = Q K^T for this warp's 32 keys, four tiles of eight
+        float sc[4][4];
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const int h = gq + 8 * half;
-        uint4 raw[4];
-        float amax = 0.f;
-        const uint4* src = reinterpret_cast<const uint4*>(
-            args.q + (static_cast<int64_t>(meta.token) * args.num_heads + meta.group * Hg + h) * 128 +
-            32 * c);
+        for (int n = 0; n < 4; ++n) {
+          const uint4 ka = lds128(st + k_off + n * 1024);
+          const uint4 kb = lds128(st + (k_off ^ 16) + n * 1024);
+          const uint32_t w[8] = {ka.x, ka.y, ka.z, ka.w, kb.x, kb.y, kb.z, kb.w};
+          sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.f;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) raw[k] = h < Hg ? __ldg(src + k) : make_uint4(0, 0, 0, 0);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const uint32_t w[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            amax = fmaxf(amax, fmaxf(fabsf(bf16_lo(w[j])), fabsf(bf16_hi(w[j]))));
+          for (int kk = 0; kk < 8; ++kk)
+            mma_f16_16816(sc[n], qa[kk], f16x2_lo(w[kk]), f16x2_hi(w[kk]));
         }
-        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-        // 2^-e with e the exponent of the row's largest value, kept to where
-        // the factor stays normal under every page scale: f16 then holds
-        // every value to 2^-25 of the largest.
-        const int e = min(max(static_cast<int>(__float_as_uint(amax) >> 23) - 127, -60), 78);
-        const float down = __int_as_float((127 - e) << 23);
-        const float factor = args.scale_log2 * __int_as_float((127 + e) << 23);
-        if (half == 0) f0 = factor; else f1 = factor;
+        // ---- keys past the limit
+        const bool ragged = seen < 32;
+        if (ragged) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const uint32_t w[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
+          for (int n = 0; n < 4; ++n)
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            qa[2 * k + (j >> 1)][half + 2 * (j & 1)] =
-                pack_f16x2(bf16_lo(w[j]) * down, bf16_hi(w[j]) * down);
+            for (int e = 0; e < 4; ++e)
+              if (n * 8 + 2 * c + (e & 1) >= seen) sc[n][e] = -INFINITY;
+        }
+        // ---- online softmax in the log2 domain
+        const float k0 = f0 * desc.k_scale, k1 = f1 * desc.k_scale, v_log2 = desc.v_log2;
+        float x0 = -INFINITY, x1 = -INFINITY;
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+          x0 = fmaxf(x0, fmaxf(sc[n][0], sc[n][1]));
+          if (!kHalf) x1 = fmaxf(x1, fmaxf(sc[n][2], sc[n][3]));
+        }
+        x0 = fmaf(x0, k0, v_log2);
+        if (!kHalf) x1 = fmaf(x1, k1, v_log2);
+        if (__any_sync(0xffffffffu, x0 > m0 + kSlack || (!kHalf && x1 > m1 + kSlack))) {
+          x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, 1));
+          x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, 2));
+          float a0 = 1.f, a1 = 1.f;
+          if (x0 > m0 + kSlack) {
+            a0 = ex2(m0 - (x0 - kHeadroom));
+            m0 = x0 - kHeadroom;
+          }
+          l0 *= a0;
+          if (!kHalf) {
+            x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, 1));
+            x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, 2));
+            if (x1 > m1 + kSlack) {
+              a1 = ex2(m1 - (x1 - kHeadroom));
+              m1 = x1 - kHeadroom;
+            }
+            l1 *= a1;
+          }
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            o[j][0] *= a0;
+            o[j][1] *= a0;
+            if (!kHalf) {
+              o[j][2] *= a1;
+              o[j][3] *= a1;
+            }
+          }
+        }
+        const float d0 = v_log2 - (m0 == -INFINITY ? 0.f : m0);
+        const float d1 = v_log2 - (m1 == -INFINITY ? 0.f : m1);
+        float sum0 = 0.f, sum1 = 0.f;
+        uint32_t pa[2][4];
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+          const float p0 = ex2(fmaf(sc[n][0], k0, d0)), p1 = ex2(fmaf(sc[n][1], k0, d0));
+          sum0 += p0 + p1;
+          pa[n >> 1][2 * (n & 1)] = pack_f16x2(p0, p1);
+          if (kHalf) {
+            pa[n >> 1][2 * (n & 1) + 1] = 0;
+          } else {
+            const float p2 = ex2(fmaf(sc[n][2], k1, d1)), p3 = ex2(fmaf(sc[n][3], k1, d1));
+            sum1 += p2 + p3;
+            pa[n >> 1][2 * (n & 1) + 1] = pack_f16x2(p2, p3);
+          }
+        }
+        l0 = fmaf(sum0, desc.v_inv, l0);
+        if (!kHalf) l1 = fmaf(sum1, desc.v_inv, l1);
+        // ---- O += P V, 16 keys at a time.  A quad lane's four keys (2c, 2c+1,
+        // 2c+8, 2c+9), 16 dims each (16 gq ..): accumulator tile j holds dim
+        // 16 n + j.
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          uint32_t vw[4][4];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const uint4 v =
+                lds128(st + ((r & 1) ? v_off1 : v_off0) + t * 2048 + (r >> 1) * 1024);
+            vw[r][0] = v.x;
+            vw[r][1] = v.y;
+            vw[r][2] = v.z;
+            vw[r][3] = v.w;
+            // Rows past the limit may hold anything, NaN codes among it.
+            if (ragged && 16 * t + 2 * c + (r & 1) + 8 * (r >> 1) >= seen)
+              vw[r][0] = vw[r][1] = vw[r][2] = vw[r][3] = 0;
+          }
+#pragma unroll
+          for (int q4 = 0; q4 < 4; ++q4) {
+            const uint32_t lo0 = __byte_perm(vw[0][q4], vw[1][q4], 0x5140);
+            const uint32_t hi0 = __byte_perm(vw[0][q4], vw[1][q4], 0x7362);
+            const uint32_t lo1 = __byte_perm(vw[2][q4], vw[3][q4], 0x5140);
+            const uint32_t hi1 = __byte_perm(vw[2][q4], vw[3][q4], 0x7362);
+            mma_f16_16816(o[4 * q4], pa[t], f16x2_lo(lo0), f16x2_lo(lo1));
+            mma_f16_16816(o[4 * q4 + 1], pa[t], f16x2_hi(lo0), f16x2_hi(lo1));
+            mma_f16_16816(o[4 * q4 + 2], pa[t], f16x2_lo(hi0), f16x2_lo(hi1));
+            mma_f16_16816(o[4 * q4 + 3], pa[t], f16x2_hi(hi0), f16x2_hi(hi1));
+          }
         }
       }
-#pragma unroll
-      for (int j = 0; j < 16; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
-      m0 = m1 = -INFINITY;
-      l0 = l1 = 0.f;
-    }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&ps->empty[slot]);
+      if (++slot == kStages) {
+        slot = 0;
+        phase ^= 1;
+      }
+    } while (!(flags & kLast));
 
-    const int page_key0 = meta.key0 + key_base;
-    if ((meta.flags & kData) && page_key0 <= meta.limit) {
-      const uint32_t st = smem_u32(stages + s * kStageBytes);
-      // ---- S = Q K^T for this warp's 16 keys, two accumulator sets a tile
-      float sc[2][4], sh[2][4];
-#pragma unroll
-      for (int n = 0; n < 2; ++n) {
-        sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.f;
-        sh[n][0] = sh[n][1] = sh[n][2] = sh[n][3] = 0.f;
-        const int key = key_base + n * 8 + gq;
-        const uint4 ka = lds128(st + sw128(key, 2 * c));
-        const uint4 kb = lds128(st + sw128(key, 2 * c + 1));
-        const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
-#pragma unroll
-        for (int kk = 0; kk < 4; ++kk) {
-          mma_f16_16816(sc[n], qa[kk], f16x2_lo(wa[kk]), f16x2_hi(wa[kk]));
-          mma_f16_16816(sh[n], qa[kk + 4], f16x2_lo(wb[kk]), f16x2_hi(wb[kk]));
-        }
-      }
-#pragma unroll
-      for (int n = 0; n < 2; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) sc[n][e] += sh[n][e];
-      // ---- keys past the limit
-      const bool ragged = page_key0 + 15 > meta.limit;
-      if (ragged) {
-#pragma unroll
-        for (int n = 0; n < 2; ++n)
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (page_key0 + n * 8 + 2 * c + (e & 1) > meta.limit) sc[n][e] = -INFINITY;
-      }
-      // ---- online softmax in the log2 domain
-      const float k0 = f0 * meta.k_scale, k1 = f1 * meta.k_scale;
-      float x0 = fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[1][0], sc[1][1])) * k0 + meta.v_log2;
-      float x1 = fmaxf(fmaxf(sc[0][2], sc[0][3]), fmaxf(sc[1][2], sc[1][3])) * k1 + meta.v_log2;
-      if (__any_sync(0xffffffffu, x0 > m0 + kSlack || x1 > m1 + kSlack)) {
-        x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, 1));
-        x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, 2));
-        x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, 1));
-        x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, 2));
-        float a0 = 1.f, a1 = 1.f;
-        if (x0 > m0 + kSlack) {
-          a0 = ex2(m0 - (x0 - kHeadroom));
-          m0 = x0 - kHeadroom;
-        }
-        if (x1 > m1 + kSlack) {
-          a1 = ex2(m1 - (x1 - kHeadroom));
-          m1 = x1 - kHeadroom;
-        }
-        l0 *= a0;
-        l1 *= a1;
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          o[j][0] *= a0;
-          o[j][1] *= a0;
-          o[j][2] *= a1;
-          o[j][3] *= a1;
-        }
-      }
-      const float d0 = meta.v_log2 - (m0 == -INFINITY ? 0.f : m0);
-      const float d1 = meta.v_log2 - (m1 == -INFINITY ? 0.f : m1);
-      float p[2][4];
-#pragma unroll
-      for (int n = 0; n < 2; ++n) {
-        p[n][0] = ex2(fmaf(sc[n][0], k0, d0));
-        p[n][1] = ex2(fmaf(sc[n][1], k0, d0));
-        p[n][2] = ex2(fmaf(sc[n][2], k1, d1));
-        p[n][3] = ex2(fmaf(sc[n][3], k1, d1));
-      }
-      l0 = fmaf((p[0][0] + p[0][1]) + (p[1][0] + p[1][1]), meta.v_inv, l0);
-      l1 = fmaf((p[0][2] + p[0][3]) + (p[1][2] + p[1][3]), meta.v_inv, l1);
-      uint32_t pa[4];
-      pa[0] = pack_f16x2(p[0][0], p[0][1]);
-      pa[1] = pack_f16x2(p[0][2], p[0][3]);
-      pa[2] = pack_f16x2(p[1][0], p[1][1]);
-      pa[3] = pack_f16x2(p[1][2], p[1][3]);
-      // ---- O += P V.  A quad lane's four keys (2c, 2c+1, 2c+8, 2c+9), 16
-      // dims each (16 gq ..): accumulator tile j holds dim 16 n + j.
-      const uint32_t vt = st + kTileBytes;
-      uint32_t vw[4][4];
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int in_warp = 2 * c + (r & 1) + 8 * (r >> 1);
-        const uint4 v = lds128(vt + sw128(key_base + in_warp, gq));
-        vw[r][0] = v.x;
-        vw[r][1] = v.y;
-        vw[r][2] = v.z;
-        vw[r][3] = v.w;
-        // Rows past the limit may hold anything, NaN codes among it.
-        if (ragged && page_key0 + in_warp > meta.limit)
-          vw[r][0] = vw[r][1] = vw[r][2] = vw[r][3] = 0;
-      }
-#pragma unroll
-      for (int q4 = 0; q4 < 4; ++q4) {
-        const uint32_t lo0 = __byte_perm(vw[0][q4], vw[1][q4], 0x5140);
-        const uint32_t hi0 = __byte_perm(vw[0][q4], vw[1][q4], 0x7362);
-        const uint32_t lo1 = __byte_perm(vw[2][q4], vw[3][q4], 0x5140);
-        const uint32_t hi1 = __byte_perm(vw[2][q4], vw[3][q4], 0x7362);
-        mma_f16_16816(o[4 * q4], pa, f16x2_lo(lo0), f16x2_lo(lo1));
-        mma_f16_16816(o[4 * q4 + 1], pa, f16x2_hi(lo0), f16x2_hi(lo1));
-        mma_f16_16816(o[4 * q4 + 2], pa, f16x2_lo(hi0), f16x2_lo(hi1));
-        mma_f16_16816(o[4 * q4 + 3], pa, f16x2_hi(hi0), f16x2_hi(hi1));
-      }
-    }
-    __syncwarp();
-    if (lane == 0) mbar_arrive(&sm->empty[s]);
-    if (!(meta.flags & kLast)) continue;
-
-    // ---- end of this CTA's share of the row: join the four warps
+    // ---- end of this range's share of the row: join the four warps
+    const int part = (flags >> 20) - 1;
+    float (*m_part)[16] = sm->m_part[row_parity];
+    float (*l_part)[16] = sm->l_part[row_parity];
+    row_parity ^= 1;
     l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
     l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
     l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
     l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
     if (c == 0) {
-      sm->m_part[warp][gq] = m0;
-      sm->m_part[warp][gq + 8] = m1;
-      sm->l_part[warp][gq] = l0;
-      sm->l_part[warp][gq + 8] = l1;
+      m_part[warp][gq] = m0;
+      m_part[warp][gq + 8] = m1;
+      l_part[warp][gq] = l0;
+      l_part[warp][gq + 8] = l1;
     }
     if (!meet()) return;
     float mt0 = -INFINITY, mt1 = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < kConsumers; ++w) {
-      mt0 = fmaxf(mt0, sm->m_part[w][gq]);
-      mt1 = fmaxf(mt1, sm->m_part[w][gq + 8]);
+    for (int w = 0; w < kWarps; ++w) {
+      mt0 = fmaxf(mt0, m_part[w][gq]);
+      mt1 = fmaxf(mt1, m_part[w][gq + 8]);
     }
     const float s0 = m0 == -INFINITY ? 0.f : ex2(m0 - mt0);
     const float s1 = m1 == -INFINITY ? 0.f : ex2(m1 - mt1);
-    // float4 i of a thread's 32 dims sits at 8c + (i ^ (c, row parity)): the
+    // float4 k of a thread's 32 dims sits at 8c + (k ^ (c, row parity)): the
     // eight lanes of a store or load phase touch eight bank groups.
-    float4* mine = reinterpret_cast<float4*>(acc) + warp * 16 * 32;
     const int swz = c | ((gq & 1) << 2);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const int e = k >> 2, j = 4 * (k & 3);
-      mine[gq * 32 + 8 * c + (k ^ swz)] = make_float4(o[j][e] * s0, o[j + 1][e] * s0,
-                                                      o[j + 2][e] * s0, o[j + 3][e] * s0);
-      mine[(gq + 8) * 32 + 8 * c + (k ^ swz)] =
-          make_float4(o[j][2 + e] * s1, o[j + 1][2 + e] * s1, o[j + 2][2 + e] * s1,
-                      o[j + 3][2 + e] * s1);
+    for (int half = 0; half < (kHalf ? 1 : 2); ++half) {
+      float4* dst = reinterpret_cast<float4*>(sums) + (warp * 16 + gq + 8 * half) * 32 + 8 * c;
+      const float f = half ? s1 : s0;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int e = 2 * half + (k >> 2), j = 4 * (k & 3);
+        dst[k ^ swz] = make_float4(o[j][e] * f, o[j + 1][e] * f, o[j + 2][e] * f, o[j + 3][e] * f);
+      }
     }
     if (!meet()) return;
     {
-      const int row = threadIdx.x >> 3, seg = threadIdx.x & 7;
+      const int row = (threadIdx.x & 127) >> 3, seg = threadIdx.x & 7;
       float mt = -INFINITY, lt = 0.f;
 #pragma unroll
-      for (int w = 0; w < kConsumers; ++w) mt = fmaxf(mt, sm->m_part[w][row]);
+      for (int w = 0; w < kWarps; ++w) mt = fmaxf(mt, m_part[w][row]);
 #pragma unroll
-      for (int w = 0; w < kConsumers; ++w)
-        lt += sm->m_part[w][row] == -INFINITY
-                  ? 0.f
-                  : sm->l_part[w][row] * ex2(sm->m_part[w][row] - mt);
-      float4 sum[4];
-      const int rswz = (seg >> 1) | ((row & 1) << 2);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        sum[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-        const int at = row * 32 + 8 * (seg >> 1) + ((4 * (seg & 1) + k) ^ rswz);
-#pragma unroll
-        for (int w = 0; w < kConsumers; ++w) {
-          const float4 x = reinterpret_cast<const float4*>(acc)[w * 16 * 32 + at];
-          sum[k].x += x.x;
-          sum[k].y += x.y;
-          sum[k].z += x.z;
-          sum[k].w += x.w;
-        }
-      }
+      for (int w = 0; w < kWarps; ++w)
+        lt += m_part[w][row] == -INFINITY ? 0.f : l_part[w][row] * ex2(m_part[w][row] - mt);
       if (row < Hg) {
-        if (meta.part >= 0) {
-          const int64_t prow = static_cast<int64_t>(meta.part) * 16 + row;
+        float4 sum[4];
+        const int rswz = (seg >> 1) | ((row & 1) << 2);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float4* src = reinterpret_cast<const float4*>(sums) + row * 32 + 8 * (seg >> 1) +
+                              ((4 * (seg & 1) + k) ^ rswz);
+          sum[k] = src[0];
+#pragma unroll
+          for (int w = 1; w < kWarps; ++w) {
+            const float4 x = src[w * 16 * 32];
+            sum[k] = make_float4(sum[k].x + x.x, sum[k].y + x.y, sum[k].z + x.z, sum[k].w + x.w);
+          }
+        }
+        if (part >= 0) {
+          const int64_t prow = static_cast<int64_t>(part) * 16 + row;
           float4* dst = reinterpret_cast<float4*>(args.part_o + prow * 128) + 4 * seg;
 #pragma unroll
           for (int k = 0; k < 4; ++k) dst[k] = sum[k];
           if (seg == 0)
             *reinterpret_cast<float2*>(args.part_ml + prow * 2) = make_float2(mt, lt);
         } else {
-          const int h = meta.group * Hg + row;
+          const int h = group * Hg + row;
           const float f = mt == -INFINITY ? 0.f : 1.f / lt;
           uint4 packed[2];
           uint32_t* pw = reinterpret_cast<uint32_t*>(packed);
@@ -674,99 +782,188 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attn_kernel(const __grid_co
             pw[2 * k + 1] = pack_bf16x2(sum[k].z * f, sum[k].w * f);
           }
           uint4* dst = reinterpret_cast<uint4*>(
-              args.out + (static_cast<int64_t>(meta.token) * args.num_heads + h) * 128 + 16 * seg);
+              args.out + (static_cast<int64_t>(token) * args.num_heads + h) * 128 + 16 * seg);
           dst[0] = packed[0];
           dst[1] = packed[1];
           if (args.lse != nullptr && seg == 0)
-            args.lse[static_cast<int64_t>(h) * args.total_q + meta.token] =
+            args.lse[static_cast<int64_t>(h) * args.total_q + token] =
                 mt == -INFINITY ? INFINITY : (mt + log2f(lt)) * 0.69314718055994531f;
         }
       }
     }
-    // The next row's partials must not overwrite what is still being read.
-    if (!meet()) return;
+    // The next row writes the other half of m_part and l_part, and `sums` only
+    // after the warps have met again.  Its first stage says which it is.
+    if (!mbar_wait(&ps->full[slot], phase, args.status, abort_flag)) return;
+    const PageDesc& next = ps->desc[stage % kDescs];
+    if (next.row & kStop) return;
+    token = next.token;
+    group = (next.row >> 4) & 0xFFFF;
   }
 }
 
 size_t paged_smem_bytes() {
-  return 1024 + kStages * kStageBytes + kConsumers * 16 * 128 * sizeof(float) + sizeof(PagedSmem);
+  return 1024 + kTeams * (kPairs * kRingBytes + kSumBytes) + sizeof(PagedSmem);
 }
 
-// Joins the parts of the row that CTA j of the attention kernel began and did
-// not finish: its second part and the first parts of CTAs j + 1 .. hi.  One
-// block per (j, head); warp w takes parts w, w + 8, ...
-constexpr int kMergeWarps = 8;
+// Writes one joined row of one head: lane l holds its dims 4l .. 4l + 3.
+__device__ __forceinline__ void write_row(const PagedAttnArgs& args, int row, int head, int lane,
+                                          float4 o, float m, float l) {
+  const float f = m == -INFINITY ? 0.f : 1.f / l;
+  const int64_t token = row / args.num_groups;
+  const int h = (row % args.num_groups) * args.heads_per_group + head;
+  uint2 packed;
+  packed.x = pack_bf16x2(o.x * f, o.y * f);
+  packed.y = pack_bf16x2(o.z * f, o.w * f);
+  reinterpret_cast<uint2*>(args.out + (token * args.num_heads + h) * 128)[lane] = packed;
+  if (args.lse != nullptr && lane == 0)
+    args.lse[static_cast<int64_t>(h) * args.total_q + token] =
+        m == -INFINITY ? INFINITY : (m + log2f(l)) * 0.69314718055994531f;
+}
 
-__global__ void __launch_bounds__(32 * kMergeWarps) paged_merge_kernel(const __grid_constant__ PagedAttnArgs args) {
-  const int j = blockIdx.x, h = blockIdx.y;
-  const int2 head = args.headers[j];
-  if (head.x < 0) return;
+// The rows cut by range borders.  A row that range j begins and does not
+// finish has its first part in the range's second workspace part; the ranges
+// behind it hold one part each (their first), up to the one whose header says
+// that the row ends there.
+__device__ __forceinline__ int64_t part_row(int j, int i, int head) {
+  return static_cast<int64_t>(i == 0 ? 2 * j + 1 : 2 * (j + i)) * 16 + head;
+}
+
+// Fewer rows than ranges (a decode step of a few long requests): a row has
+// many parts.  One block per (row, head); warp w sums parts w, w + 16, ...
+constexpr int kMergeWarps = 16;
+
+__global__ void __launch_bounds__(32 * kMergeWarps) paged_merge_many_kernel(
+    const __grid_constant__ PagedAttnArgs args, int ranges) {
   __shared__ float4 sum[kMergeWarps][32];
-  __shared__ float m_w[kMergeWarps], l_w[kMergeWarps];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int n = head.y - j + 1;
-  float m = -INFINITY, l = 0.f;
+  __shared__ float weight[kPagedMaxRanges];
+  __shared__ float warp_m[kMergeWarps], warp_l[kMergeWarps];
+  __shared__ int first, behind;
+  static_assert(kPagedMaxRanges <= 32 * kMergeWarps, "one thread per range");
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int row = blockIdx.x, h = blockIdx.y;
+  if (tid == 0) first = behind = ranges;
+  __syncthreads();
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int2 head = tid < ranges ? args.headers[tid] : make_int2(-1, 1);
+  if (head.x == row) first = tid;
+  __syncthreads();
+  const int j = first;
+  if (j >= ranges) return;  // the row is whole in one range
+  if (tid > j && tid < ranges && head.y != 0) atomicMin(&behind, tid);
+  __syncthreads();
+  const int n = min(behind, ranges - 1) - j + 1;
+  const float2 ml = tid < n ? reinterpret_cast<const float2*>(args.part_ml)[part_row(j, tid, h)]
+                            : make_float2(-INFINITY, 0.f);
+  float m = ml.x;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  if (lane == 0) warp_m[warp] = m;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kMergeWarps; ++w) m = fmaxf(m, warp_m[w]);
+  const float mine = ml.x == -INFINITY ? 0.f : ex2(ml.x - m);
+  if (tid < n) weight[tid] = mine;
+  float l = ml.y * mine;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+  if (lane == 0) warp_l[warp] = l;
+  __syncthreads();
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
+#pragma unroll 10
   for (int i = warp; i < n; i += kMergeWarps) {
-    const int64_t part = i == 0 ? 2 * j + 1 : 2 * (j + i);
-    const int64_t prow = part * 16 + h;
-    const float2 ml = *reinterpret_cast<const float2*>(args.part_ml + prow * 2);
-    const float4 x = reinterpret_cast<const float4*>(args.part_o + prow * 128)[lane];
-    if (ml.x == -INFINITY) continue;
-    const float mx = fmaxf(m, ml.x);
-    const float a = m == -INFINITY ? 0.f : ex2(m - mx), b = ex2(ml.x - mx);
-    acc.x = acc.x * a + x.x * b;
-    acc.y = acc.y * a + x.y * b;
-    acc.z = acc.z * a + x.z * b;
-    acc.w = acc.w * a + x.w * b;
-    l = l * a + ml.y * b;
-    m = mx;
+    const float w = weight[i];
+    const float4 x = reinterpret_cast<const float4*>(args.part_o + part_row(j, i, h) * 128)[lane];
+    acc.x = fmaf(x.x, w, acc.x);
+    acc.y = fmaf(x.y, w, acc.y);
+    acc.z = fmaf(x.z, w, acc.z);
+    acc.w = fmaf(x.w, w, acc.w);
   }
   sum[warp][lane] = acc;
-  if (lane == 0) {
-    m_w[warp] = m;
-    l_w[warp] = l;
-  }
   __syncthreads();
   if (warp != 0) return;
-  float mt = -INFINITY, lt = 0.f;
+  l = 0.f;
 #pragma unroll
-  for (int w = 0; w < kMergeWarps; ++w) mt = fmaxf(mt, m_w[w]);
-  float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int w = 0; w < kMergeWarps; ++w) l += warp_l[w];
+  float4 t = sum[0][lane];
 #pragma unroll
-  for (int w = 0; w < kMergeWarps; ++w) {
-    if (m_w[w] == -INFINITY) continue;
-    const float a = ex2(m_w[w] - mt);
+  for (int w = 1; w < kMergeWarps; ++w) {
     const float4 x = sum[w][lane];
-    t.x = fmaf(x.x, a, t.x);
-    t.y = fmaf(x.y, a, t.y);
-    t.z = fmaf(x.z, a, t.z);
-    t.w = fmaf(x.w, a, t.w);
-    lt = fmaf(l_w[w], a, lt);
+    t = make_float4(t.x + x.x, t.y + x.y, t.z + x.z, t.w + x.w);
   }
-  const float f = mt == -INFINITY ? 0.f : 1.f / lt;
-  const int64_t token = head.x / args.num_groups;
-  const int hh = (head.x % args.num_groups) * args.heads_per_group + h;
-  uint2 packed;
-  packed.x = pack_bf16x2(t.x * f, t.y * f);
-  packed.y = pack_bf16x2(t.z * f, t.w * f);
-  reinterpret_cast<uint2*>(args.out + (token * args.num_heads + hh) * 128)[lane] = packed;
-  if (args.lse != nullptr && lane == 0)
-    args.lse[static_cast<int64_t>(hh) * args.total_q + token] =
-        mt == -INFINITY ? INFINITY : (mt + log2f(lt)) * 0.69314718055994531f;
+  write_row(args, row, h, lane, t, m, l);
+}
+
+// At least as many rows as ranges: a cut row has two parts, seldom more.  One
+// warp per (range, head).
+__global__ void __launch_bounds__(256) paged_merge_few_kernel(
+    const __grid_constant__ PagedAttnArgs args, int ranges) {
+  const int j = blockIdx.x, lane = threadIdx.x & 31;
+  const int h = blockIdx.y * 8 + (threadIdx.x >> 5);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (h >= args.heads_per_group) return;
+  const int row = args.headers[j].x;
+  if (row < 0) return;
+  float m = -INFINITY, l = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i = 0; j + i < ranges; ++i) {
+    const int64_t at = part_row(j, i, h);
+    const float2 ml = reinterpret_cast<const float2*>(args.part_ml)[at];
+    const float4 x = reinterpret_cast<const float4*>(args.part_o + at * 128)[lane];
+    const bool last = i > 0 && args.headers[j + i].y != 0;
+    if (ml.x != -INFINITY) {
+      const float mx = fmaxf(m, ml.x);
+      const float a = m == -INFINITY ? 0.f : ex2(m - mx), b = ex2(ml.x - mx);
+      acc = make_float4(acc.x * a + x.x * b, acc.y * a + x.y * b, acc.z * a + x.z * b,
+                        acc.w * a + x.w * b);
+      l = l * a + ml.y * b;
+      m = mx;
+    }
+    if (last) break;
+  }
+  write_row(args, row, h, lane, acc, m, l);
 }
 
 }  // namespace
 
-cudaError_t launch_paged_attn(const PagedAttnArgs& args, int ctas, cudaStream_t stream) {
-  const size_t smem = paged_smem_bytes();
-  const cudaError_t err = cudaFuncSetAttribute(
-      paged_attn_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+// The register split of the kernel draws on what the block is launched with:
+// a build that gives it fewer registers must not run.
+template <bool kHalf>
+cudaError_t launch_attn_kernel(const PagedAttnArgs& args, int ranges, cudaStream_t stream) {
+  cudaFuncAttributes attr;
+  cudaError_t err = cudaFuncGetAttributes(&attr, paged_attn_kernel<kHalf>);
   if (err != cudaSuccess) return err;
-  paged_attn_kernel<<<ctas, kThreads, smem, stream>>>(args);
-  paged_merge_kernel<<<dim3(ctas, args.heads_per_group), 32 * kMergeWarps, 0, stream>>>(args);
-  return cudaGetLastError();
+  if (attr.numRegs != kLaunchRegs) return cudaErrorInvalidConfiguration;
+  const size_t smem = paged_smem_bytes();
+  err = cudaFuncSetAttribute(paged_attn_kernel<kHalf>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             static_cast<int>(smem));
+  if (err != cudaSuccess) return err;
+  const int ctas = (ranges + kTeams - 1) / kTeams;
+  paged_attn_kernel<kHalf><<<ctas, kThreads, smem, stream>>>(args);
+  err = cudaGetLastError();
+  if (err != cudaSuccess) return err;
+  const int64_t rows = args.total_q * args.num_groups;
+  ranges = ctas * kTeams;
+  // The merge is set up while the attention runs and waits for its end.
+  cudaLaunchAttribute early;
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.stream = stream;
+  cfg.attrs = &early;
+  cfg.numAttrs = 1;
+  if (rows < ranges) {
+    cfg.gridDim = dim3(static_cast<unsigned>(rows), args.heads_per_group);
+    cfg.blockDim = dim3(32 * kMergeWarps);
+    return cudaLaunchKernelEx(&cfg, paged_merge_many_kernel, args, ranges);
+  }
+  cfg.gridDim = dim3(ranges, (args.heads_per_group + 7) / 8);
+  cfg.blockDim = dim3(256);
+  return cudaLaunchKernelEx(&cfg, paged_merge_few_kernel, args, ranges);
+}
+
+cudaError_t launch_paged_attn(const PagedAttnArgs& args, int ranges, cudaStream_t stream) {
+  return args.heads_per_group <= 8 ? launch_attn_kernel<true>(args, ranges, stream)
+                                   : launch_attn_kernel<false>(args, ranges, stream);
 }
 
 }  // namespace ls
