@@ -828,7 +828,7 @@ __device__ __forceinline__ int64_t part_row(int j, int i, int head) {
   return static_cast<int64_t>(i == 0 ? 2 * j + 1 : 2 * (j + i)) * 16 + head;
 }
 
-// Fewer rows than ranges (a decode step of a few long requests): a row has
+// Far fewer rows than ranges (a decode step of a few long requests): a row has
 // many parts.  One block per (row, head); warp w sums parts w, w + 16, ...
 constexpr int kMergeWarps = 16;
 
@@ -893,8 +893,8 @@ __global__ void __launch_bounds__(32 * kMergeWarps) paged_merge_many_kernel(
   write_row(args, row, h, lane, t, m, l);
 }
 
-// At least as many rows as ranges: a cut row has two parts, seldom more.  One
-// warp per (range, head).
+// Otherwise most cut rows have a few parts.  One warp per (range, head); lane
+// i looks after part i of 32 at a time.
 __global__ void __launch_bounds__(256) paged_merge_few_kernel(
     const __grid_constant__ PagedAttnArgs args, int ranges) {
   const int j = blockIdx.x, lane = threadIdx.x & 31;
@@ -905,21 +905,36 @@ __global__ void __launch_bounds__(256) paged_merge_few_kernel(
   if (row < 0) return;
   float m = -INFINITY, l = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int i = 0; j + i < ranges; ++i) {
-    const int64_t at = part_row(j, i, h);
-    const float2 ml = reinterpret_cast<const float2*>(args.part_ml)[at];
-    const float4 x = reinterpret_cast<const float4*>(args.part_o + at * 128)[lane];
-    const bool last = i > 0 && args.headers[j + i].y != 0;
-    if (ml.x != -INFINITY) {
-      const float mx = fmaxf(m, ml.x);
-      const float a = m == -INFINITY ? 0.f : ex2(m - mx), b = ex2(ml.x - mx);
-      acc = make_float4(acc.x * a + x.x * b, acc.y * a + x.y * b, acc.z * a + x.z * b,
-                        acc.w * a + x.w * b);
-      l = l * a + ml.y * b;
-      m = mx;
+  bool more = true;
+  for (int base = 0; more; base += 32) {
+    const int k = j + base + lane;
+    const uint32_t ends =
+        __ballot_sync(0xffffffffu, k >= ranges || (base + lane > 0 && args.headers[k].y != 0));
+    more = ends == 0;
+    int n = more ? 32 : __ffs(ends);
+    if (j + base + n > ranges) n = ranges - j - base;
+    const float2 ml = lane < n ? reinterpret_cast<const float2*>(
+                                     args.part_ml)[part_row(j, base + lane, h)]
+                               : make_float2(-INFINITY, 0.f);
+    float mx = fmaxf(m, ml.x);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    const float keep = m == -INFINITY ? 0.f : ex2(m - mx);
+    const float w = ml.x == -INFINITY ? 0.f : ex2(ml.x - mx);
+    m = mx;
+    l = fmaf(l, keep, ml.y * w);  // a lane's share; summed at the end
+    acc = make_float4(acc.x * keep, acc.y * keep, acc.z * keep, acc.w * keep);
+#pragma unroll 4
+    for (int i = 0; i < n; ++i) {
+      const float wi = __shfl_sync(0xffffffffu, w, i);
+      const float4 x =
+          reinterpret_cast<const float4*>(args.part_o + part_row(j, base + i, h) * 128)[lane];
+      acc = make_float4(fmaf(x.x, wi, acc.x), fmaf(x.y, wi, acc.y), fmaf(x.z, wi, acc.z),
+                        fmaf(x.w, wi, acc.w));
     }
-    if (last) break;
   }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
   write_row(args, row, h, lane, acc, m, l);
 }
 
@@ -951,7 +966,7 @@ cudaError_t launch_attn_kernel(const PagedAttnArgs& args, int ranges, cudaStream
   cfg.stream = stream;
   cfg.attrs = &early;
   cfg.numAttrs = 1;
-  if (rows < ranges) {
+  if (rows * 16 < ranges) {  // more than 16 parts a row
     cfg.gridDim = dim3(static_cast<unsigned>(rows), args.heads_per_group);
     cfg.blockDim = dim3(32 * kMergeWarps);
     return cudaLaunchKernelEx(&cfg, paged_merge_many_kernel, args, ranges);
