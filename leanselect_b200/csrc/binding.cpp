@@ -68,6 +68,15 @@ bool token_rows(const Tensor* t, int dev, int64_t g, int64_t d) {
          t->stride(0) >= g * d && reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0;
 }
 
+// Elements [from, from + n) of this type in a buffer, as a vector sharing its storage.
+Tensor slice(const Tensor& buffer, at::ScalarType type, int64_t from, int64_t n) {
+  auto impl = c10::make_intrusive<at::TensorImpl>(
+      c10::Storage(buffer.storage()), buffer.key_set(), c10::scalarTypeToTypeMeta(type));
+  impl->set_storage_offset(from);
+  impl->set_sizes_contiguous({n});
+  return Tensor(std::move(impl));
+}
+
 bool fits32(int64_t x) { return x >= 0 && x < (int64_t{1} << 31); }
 
 // plan_pages(context_lens, new_lens, block_table, free_pages, free_head, total_new, status)
@@ -93,27 +102,28 @@ PyObject* plan_pages(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   at::AutoDispatchBelowADInplaceOrView below;
   const c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(dev));
   const auto opts = at::TensorOptions().device(at::kCUDA, static_cast<c10::DeviceIndex>(dev));
-  // Two allocations: int32 results, and slots and positions (each 16-byte aligned).
-  const Tensor ints = at::empty({3 * batch + 3}, opts.dtype(at::kInt));
-  const int64_t even = (total + 1) / 2 * 2;
-  const Tensor longs = at::empty({2 * even}, opts.dtype(at::kLong));
-  int32_t* i = ints.data_ptr<int32_t>();
-  int64_t* l = even ? longs.data_ptr<int64_t>() : nullptr;
+  // One allocation: slots, positions (each 16-byte aligned), then the int32 results.
+  const int64_t even = (total + 1) / 2 * 2, ints = 4 * even;
+  const Tensor buffer = at::empty({16 * even + 4 * (3 * batch + 3)}, opts.dtype(at::kByte));
+  int64_t* l = static_cast<int64_t*>(buffer.data_ptr());
+  int32_t* i = reinterpret_cast<int32_t*>(l + 2 * even);
   void* stream = c10::cuda::getCurrentCUDAStream(static_cast<c10::DeviceIndex>(dev)).stream();
   int rc;
   Py_BEGIN_ALLOW_THREADS
   rc = ls_plan_pages(ptr<int32_t>(ctx), ptr<int32_t>(add), static_cast<int32_t>(batch),
                      ptr<int32_t>(table), static_cast<int32_t>(table->size(1)), ptr<int32_t>(pool),
                      static_cast<int32_t>(pool->size(0)), ptr<int32_t>(head), total, i, i + batch,
-                     i + 2 * batch + 1, l, even ? l + even : nullptr, i + 3 * batch + 2,
+                     i + 2 * batch + 1, l, l + even, i + 3 * batch + 2,
                      ptr<int32_t>(status), stream);
   Py_END_ALLOW_THREADS
-  return Py_BuildValue(
-      "(iNNNNNN)", rc, THPVariable_Wrap(ints.narrow(0, 0, batch)),
-      THPVariable_Wrap(ints.narrow(0, batch, batch + 1)),
-      THPVariable_Wrap(ints.narrow(0, 2 * batch + 1, batch + 1)),
-      THPVariable_Wrap(longs.narrow(0, 0, total)), THPVariable_Wrap(longs.narrow(0, even, total)),
-      THPVariable_Wrap(ints.narrow(0, 3 * batch + 2, 1)));
+  const auto vec32 = [&](int64_t from, int64_t n) {
+    return THPVariable_Wrap(slice(buffer, at::kInt, ints + from, n));
+  };
+  return Py_BuildValue("(iNNNNNN)", rc, vec32(0, batch), vec32(batch, batch + 1),
+                       vec32(2 * batch + 1, batch + 1),
+                       THPVariable_Wrap(slice(buffer, at::kLong, 0, total)),
+                       THPVariable_Wrap(slice(buffer, at::kLong, even, total)),
+                       vec32(3 * batch + 2, 1));
   END_HANDLE_TH_ERRORS
 }
 

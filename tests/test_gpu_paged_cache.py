@@ -230,6 +230,39 @@ def test_append(context, new, G):
     run_append(context, new, G, k, v, cache, table)
 
 
+@pytest.mark.parametrize("batch, kind", [(33, "one"), (300, "one"), (300, "sparse"),
+                                         (1200, "sparse"), (90, "ragged"), (1100, "late")])
+def test_append_finds_the_request_of_every_page(batch, kind):
+    """Batches beyond one probe of 32 requests: a token each, few requests with
+    tokens, requests of many pages, and all tokens in the last requests."""
+    gen = torch.Generator().manual_seed(batch)
+    context = torch.randint(0, 100, (batch,), generator=gen).tolist()
+    if kind == "one":
+        new = [1] * batch
+    elif kind == "sparse":
+        new = [(b % 61 == 7) * (1 + b % 3) for b in range(batch)]
+    elif kind == "late":
+        new = [0] * (batch - 5) + [70, 0, 3, 200, 1]
+    else:
+        new = [(b * 37) % 150 for b in range(batch)]
+    need = [up(c + n) for c, n in zip(context, new)]
+    table, _ = first_table([c + n for c, n in zip(context, new)], max(need), sum(need) + 4, gen)
+    k = torch.randn(sum(new), 1, 128, generator=gen).bfloat16().to(DEV)
+    run_append(context, new, 1, k, -k, empty_cache(sum(need) + 4, 1, 3), table)
+
+
+def test_append_offsets_that_are_no_prefix_sums_are_reported():
+    """Bad block offsets end the search and write nothing out of range."""
+    cache = empty_cache(3, 1, 1)
+    k = torch.zeros(100, 1, 128, dtype=torch.bfloat16, device=DEV)
+    for cu_blocks in ([5] * 100 + [7], [0] * 50 + [90] * 50 + [8], list(range(100, -1, -1))):
+        plan = ops.PagePlan(i32([0] * 100), i32([1] * 100), i32(list(range(101))),
+                            i32(cu_blocks), torch.zeros(100, dtype=torch.int64, device=DEV), None)
+        ops.append_kv(k, k, plan, *cache)
+        torch.cuda.synchronize()
+        ops.status_word(DEV).zero_()
+
+
 def test_append_extremes():
     """Zeros, subnormals, values at and next to 448 s, infinities and NaN."""
     gen = torch.Generator().manual_seed(5)
