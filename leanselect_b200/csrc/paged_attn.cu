@@ -23,8 +23,9 @@
 // parts of a row cut by range borders go to a workspace and
 // paged_merge_kernel joins them.  The cut depends on the shapes and lengths
 // alone, and no sum uses atomics, so equal calls give equal bits.
+#include <atomic>
+
 #include <cuda_fp16.h>
-#include <cuda_fp8.h>
 
 #include "common.cuh"
 #include "launch.h"
@@ -940,20 +941,34 @@ __global__ void __launch_bounds__(256) paged_merge_few_kernel(
 
 }  // namespace
 
-// The register split of the kernel draws on what the block is launched with:
-// a build that gives it fewer registers must not run.
+// Once per device: the register split of the kernel draws on what the block is
+// launched with, so a build that gives it fewer registers must not run; and the
+// shared memory limit.
 template <bool kHalf>
-cudaError_t launch_attn_kernel(const PagedAttnArgs& args, int ranges, cudaStream_t stream) {
+cudaError_t prepare_attn_kernel() {
+  static std::atomic<uint64_t> ready[4];  // a bit per device, set once it is done there
+  int device = 0;
+  cudaError_t err = cudaGetDevice(&device);
+  if (err != cudaSuccess) return err;
+  const uint64_t bit = uint64_t{1} << (device & 63);
+  const bool tracked = device >= 0 && device < 256;
+  if (tracked && (ready[device >> 6].load(std::memory_order_acquire) & bit)) return cudaSuccess;
   cudaFuncAttributes attr;
-  cudaError_t err = cudaFuncGetAttributes(&attr, paged_attn_kernel<kHalf>);
+  err = cudaFuncGetAttributes(&attr, paged_attn_kernel<kHalf>);
   if (err != cudaSuccess) return err;
   if (attr.numRegs != kLaunchRegs) return cudaErrorInvalidConfiguration;
-  const size_t smem = paged_smem_bytes();
   err = cudaFuncSetAttribute(paged_attn_kernel<kHalf>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             static_cast<int>(smem));
+                             static_cast<int>(paged_smem_bytes()));
+  if (err == cudaSuccess && tracked) ready[device >> 6].fetch_or(bit, std::memory_order_release);
+  return err;
+}
+
+template <bool kHalf>
+cudaError_t launch_attn_kernel(const PagedAttnArgs& args, int ranges, cudaStream_t stream) {
+  cudaError_t err = prepare_attn_kernel<kHalf>();
   if (err != cudaSuccess) return err;
   const int ctas = (ranges + kTeams - 1) / kTeams;
-  paged_attn_kernel<kHalf><<<ctas, kThreads, smem, stream>>>(args);
+  paged_attn_kernel<kHalf><<<ctas, kThreads, paged_smem_bytes(), stream>>>(args);
   err = cudaGetLastError();
   if (err != cudaSuccess) return err;
   const int64_t rows = args.total_q * args.num_groups;
