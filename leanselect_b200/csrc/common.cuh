@@ -232,6 +232,22 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
 }
 
 // ---------------------------------------------------------------------------
+// Programmatic dependent launch
+// ---------------------------------------------------------------------------
+
+// Until the grids this one depends on have finished and their writes are
+// seen: before the first access to global memory of a kernel launched early.
+__device__ __forceinline__ void wait_for_inputs() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
+// Lets the next kernel of the stream be set up once every CTA has got here; it
+// still waits for this grid's end if it was launched early, as above.
+__device__ __forceinline__ void allow_next_launch() {
+  asm volatile("griddepcontrol.launch_dependents;");
+}
+
+// ---------------------------------------------------------------------------
 // Small numeric helpers
 // ---------------------------------------------------------------------------
 

@@ -126,6 +126,24 @@ cudaError_t launch_sparse_attn_merge(const AttnArgs& args, cudaStream_t stream);
 // the attention kernel cannot beat (a measured roofline for it).
 cudaError_t launch_sparse_attn_gather_only(const AttnArgs& args, cudaStream_t stream);
 
+// Launches a kernel that may be set up while the stream's previous kernel
+// still runs; the kernel calls wait_for_inputs() before it touches memory.
+template <typename... Params, typename... Args>
+cudaError_t launch_early(void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem,
+                         cudaStream_t stream, Args... args) {
+  cudaLaunchAttribute early;
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cfg.attrs = &early;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
+}
+
 // Page planning and cache write of the 8-bit paged cache (paged_cache.cu).
 struct PlanArgs {
   const int32_t* context_lens;

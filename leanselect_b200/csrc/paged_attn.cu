@@ -107,6 +107,33 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// mbar_wait for warps that wait often and long: the thread is suspended for up
+// to 20 us a try, so that it takes no issue slots from the warps it waits for.
+__device__ __forceinline__ bool mbar_sleep(uint64_t* bar, uint32_t parity, int32_t* status,
+                                           volatile int* abort_flag) {
+  const uint32_t addr = smem_u32(bar);
+  uint64_t start = 0;
+  while (true) {
+    uint32_t ok = 0;
+    asm volatile(
+        "{\n\t.reg .pred P;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 P, [%1], %2, %3;\n\t"
+        "selp.b32 %0, 1, 0, P;\n\t}"
+        : "=r"(ok)
+        : "r"(addr), "r"(parity), "r"(20000)
+        : "memory");
+    if (ok) return true;
+    if (*abort_flag) return false;
+    const uint64_t now = globaltimer();
+    if (start == 0) start = now;
+    if (now - start > LS_WAIT_TIMEOUT_NS) {
+      report(status, LS_DEVERR_TIMEOUT);
+      *abort_flag = 1;
+      return false;
+    }
+  }
+}
+
 // Two e4m3 codes (the low or the high half of a word) as f16x2.
 __device__ __forceinline__ uint32_t f16x2_lo(uint32_t w) {
   uint32_t d;
@@ -193,6 +220,46 @@ __device__ __forceinline__ void load_query(const uint16_t* q, int gq, int heads,
   }
 }
 
+// B fragments of 16 keys' values in f16.  A quad lane's four keys (2c, 2c + 1,
+// 2c + 8, 2c + 9) are read 16 dims each (16 gq ..); tile j holds dim 16 n + j.
+// Keys past the row's limit (`seen` of the warp's 32) may hold anything, NaN
+// codes among it, and count as zeros.
+__device__ __forceinline__ void load_values(uint32_t stage, uint32_t off0, uint32_t off1, int t,
+                                            int c, int seen, uint32_t (&vb)[16][2]) {
+  uint32_t w[4][4];
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const uint4 v = lds128(stage + ((r & 1) ? off1 : off0) + t * 2048 + (r >> 1) * 1024);
+    w[r][0] = v.x;
+    w[r][1] = v.y;
+    w[r][2] = v.z;
+    w[r][3] = v.w;
+  }
+  if (seen < 32) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (16 * t + 2 * c + (r & 1) + 8 * (r >> 1) >= seen) w[r][0] = w[r][1] = w[r][2] = w[r][3] = 0;
+  }
+#pragma unroll
+  for (int q4 = 0; q4 < 4; ++q4) {
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const uint32_t lo = __byte_perm(w[2 * half][q4], w[2 * half + 1][q4], 0x5140);
+      const uint32_t hi = __byte_perm(w[2 * half][q4], w[2 * half + 1][q4], 0x7362);
+      vb[4 * q4][half] = f16x2_lo(lo);
+      vb[4 * q4 + 1][half] = f16x2_hi(lo);
+      vb[4 * q4 + 2][half] = f16x2_lo(hi);
+      vb[4 * q4 + 3][half] = f16x2_hi(hi);
+    }
+  }
+}
+
+__device__ __forceinline__ void mma_values(float (&o)[16][4], const uint32_t (&p)[4],
+                                           const uint32_t (&vb)[16][2]) {
+#pragma unroll
+  for (int j = 0; j < 16; ++j) mma_f16_16816(o[j], p, vb[j][0], vb[j][1]);
+}
+
 // Byte offset of 16-byte chunk `chunk` (0..7) of row `row` in a 128B-swizzled box.
 __device__ __forceinline__ uint32_t sw128(int row, int chunk) {
   return static_cast<uint32_t>(row * 128 + ((chunk ^ (row & 7)) << 4));
@@ -243,8 +310,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
   PagedSmem* shared =
       reinterpret_cast<PagedSmem*>(smem + kTeams * (kPairs * kRingBytes + kSumBytes));
 
-  // The merge kernel may be set up from now on; it waits for this grid's end.
-  asm volatile("griddepcontrol.launch_dependents;");
+  allow_next_launch();  // the merge: it waits for this grid's end
 
   const int warp_id = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -262,6 +328,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
     t->abort_flag = 0;
     fence_barrier_init();
   }
+
+  wait_for_inputs();
 
   // ---- the work of all rows, and where the teams' ranges start
   // listed: row r = (group, token) has `topk` units, ordered group-major.
@@ -451,7 +519,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
 #pragma unroll
           for (int j = 0; j < kStages; ++j) {
             if (j < early && ok) {
-              ok = mbar_wait(&ps->empty[s0], p0, args.status, abort_flag);
+              ok = mbar_sleep(&ps->empty[s0], p0, args.status, abort_flag);
               if (ok && y0[j] >= 0) {
                 mbar_expect_tx(&ps->full[s0], kStageBytes);
                 load_page(args, ring + s0 * kStageBytes, &ps->full[s0], y0[j]);
@@ -481,7 +549,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
               // also after a wait that gave up: what is in flight may land
               mbar_arrive(&ps->full[slot]);
             } else {
-              ok = ok && mbar_wait(&ps->empty[slot], phase, args.status, abort_flag);
+              ok = ok && mbar_sleep(&ps->empty[slot], phase, args.status, abort_flag);
               if (!ok) break;
               const int y = ps->desc[(fill + j) % kDescs].y;
               if (y >= 0) {
@@ -521,7 +589,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
       }
     }
     if (lane == 0) {
-      if (ok) ok = mbar_wait(&ps->empty[slot], phase, args.status, abort_flag);
+      if (ok) ok = mbar_sleep(&ps->empty[slot], phase, args.status, abort_flag);
       if (ok) {
         ps->desc[fill % kDescs].row = kStop;
         mbar_arrive(&ps->full[slot]);
@@ -563,7 +631,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
   auto meet = [&]() {
     __syncwarp();
     if (lane == 0) mbar_arrive(&sm->join);
-    return mbar_wait(&sm->join, joins++ & 1, args.status, abort_flag);
+    return mbar_sleep(&sm->join, joins++ & 1, args.status, abort_flag);
   };
 
   int slot = 0, stage = 0, row_parity = 0;
@@ -580,7 +648,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
     float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
     int flags;
     do {
-      if (!mbar_wait(&ps->full[slot], phase, args.status, abort_flag)) return;
+      if (!mbar_sleep(&ps->full[slot], phase, args.status, abort_flag)) return;
       const PageDesc& desc = ps->desc[stage++ % kDescs];
       flags = desc.row;
 
@@ -600,6 +668,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
           for (int kk = 0; kk < 8; ++kk)
             mma_f16_16816(sc[n], qa[kk], f16x2_lo(w[kk]), f16x2_hi(w[kk]));
         }
+        // The values of the first 16 keys are converted while the products run.
+        uint32_t vb[16][2];
+        load_values(st, v_off0, v_off1, 0, c, seen, vb);
         // ---- keys past the limit
         const bool ragged = seen < 32;
         if (ragged) {
@@ -666,36 +737,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
         }
         l0 = fmaf(sum0, desc.v_inv, l0);
         if (!kHalf) l1 = fmaf(sum1, desc.v_inv, l1);
-        // ---- O += P V, 16 keys at a time.  A quad lane's four keys (2c, 2c+1,
-        // 2c+8, 2c+9), 16 dims each (16 gq ..): accumulator tile j holds dim
-        // 16 n + j.
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          uint32_t vw[4][4];
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const uint4 v =
-                lds128(st + ((r & 1) ? v_off1 : v_off0) + t * 2048 + (r >> 1) * 1024);
-            vw[r][0] = v.x;
-            vw[r][1] = v.y;
-            vw[r][2] = v.z;
-            vw[r][3] = v.w;
-            // Rows past the limit may hold anything, NaN codes among it.
-            if (ragged && 16 * t + 2 * c + (r & 1) + 8 * (r >> 1) >= seen)
-              vw[r][0] = vw[r][1] = vw[r][2] = vw[r][3] = 0;
-          }
-#pragma unroll
-          for (int q4 = 0; q4 < 4; ++q4) {
-            const uint32_t lo0 = __byte_perm(vw[0][q4], vw[1][q4], 0x5140);
-            const uint32_t hi0 = __byte_perm(vw[0][q4], vw[1][q4], 0x7362);
-            const uint32_t lo1 = __byte_perm(vw[2][q4], vw[3][q4], 0x5140);
-            const uint32_t hi1 = __byte_perm(vw[2][q4], vw[3][q4], 0x7362);
-            mma_f16_16816(o[4 * q4], pa[t], f16x2_lo(lo0), f16x2_lo(lo1));
-            mma_f16_16816(o[4 * q4 + 1], pa[t], f16x2_hi(lo0), f16x2_hi(lo1));
-            mma_f16_16816(o[4 * q4 + 2], pa[t], f16x2_lo(hi0), f16x2_lo(hi1));
-            mma_f16_16816(o[4 * q4 + 3], pa[t], f16x2_hi(hi0), f16x2_hi(hi1));
-          }
-        }
+        // ---- O += P V, the other 16 keys converted behind the first product
+        mma_values(o, pa[0], vb);
+        load_values(st, v_off0, v_off1, 1, c, seen, vb);
+        mma_values(o, pa[1], vb);
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&ps->empty[slot]);
@@ -794,7 +839,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
     }
     // The next row writes the other half of m_part and l_part, and `sums` only
     // after the warps have met again.  Its first stage says which it is.
-    if (!mbar_wait(&ps->full[slot], phase, args.status, abort_flag)) return;
+    if (!mbar_sleep(&ps->full[slot], phase, args.status, abort_flag)) return;
     const PageDesc& next = ps->desc[stage % kDescs];
     if (next.row & kStop) return;
     token = next.token;
@@ -844,7 +889,8 @@ __global__ void __launch_bounds__(32 * kMergeWarps) paged_merge_many_kernel(
   const int row = blockIdx.x, h = blockIdx.y;
   if (tid == 0) first = behind = ranges;
   __syncthreads();
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  allow_next_launch();
+  wait_for_inputs();
   const int2 head = tid < ranges ? args.headers[tid] : make_int2(-1, 1);
   if (head.x == row) first = tid;
   __syncthreads();
@@ -900,7 +946,8 @@ __global__ void __launch_bounds__(256) paged_merge_few_kernel(
     const __grid_constant__ PagedAttnArgs args, int ranges) {
   const int j = blockIdx.x, lane = threadIdx.x & 31;
   const int h = blockIdx.y * 8 + (threadIdx.x >> 5);
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  allow_next_launch();
+  wait_for_inputs();
   if (h >= args.heads_per_group) return;
   const int row = args.headers[j].x;
   if (row < 0) return;
@@ -968,27 +1015,17 @@ cudaError_t launch_attn_kernel(const PagedAttnArgs& args, int ranges, cudaStream
   cudaError_t err = prepare_attn_kernel<kHalf>();
   if (err != cudaSuccess) return err;
   const int ctas = (ranges + kTeams - 1) / kTeams;
-  paged_attn_kernel<kHalf><<<ctas, kThreads, paged_smem_bytes(), stream>>>(args);
-  err = cudaGetLastError();
+  err = launch_early(paged_attn_kernel<kHalf>, dim3(ctas), dim3(kThreads), paged_smem_bytes(),
+                     stream, args);
   if (err != cudaSuccess) return err;
   const int64_t rows = args.total_q * args.num_groups;
+  const int heads = args.heads_per_group;
   ranges = ctas * kTeams;
-  // The merge is set up while the attention runs and waits for its end.
-  cudaLaunchAttribute early;
-  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  early.val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t cfg{};
-  cfg.stream = stream;
-  cfg.attrs = &early;
-  cfg.numAttrs = 1;
-  if (rows * 16 < ranges) {  // more than 16 parts a row
-    cfg.gridDim = dim3(static_cast<unsigned>(rows), args.heads_per_group);
-    cfg.blockDim = dim3(32 * kMergeWarps);
-    return cudaLaunchKernelEx(&cfg, paged_merge_many_kernel, args, ranges);
-  }
-  cfg.gridDim = dim3(ranges, (args.heads_per_group + 7) / 8);
-  cfg.blockDim = dim3(256);
-  return cudaLaunchKernelEx(&cfg, paged_merge_few_kernel, args, ranges);
+  if (rows * 16 < ranges)  // more than 16 parts a row
+    return launch_early(paged_merge_many_kernel, dim3(static_cast<unsigned>(rows), heads),
+                        dim3(32 * kMergeWarps), 0, stream, args, ranges);
+  return launch_early(paged_merge_few_kernel, dim3(ranges, (heads + 7) / 8), dim3(256), 0, stream,
+                      args, ranges);
 }
 
 cudaError_t launch_paged_attn(const PagedAttnArgs& args, int ranges, cudaStream_t stream) {

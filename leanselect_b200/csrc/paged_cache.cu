@@ -68,6 +68,8 @@ __global__ void __launch_bounds__(kPlanThreads) plan_pages_kernel(const __grid_c
   __shared__ uint64_t warp_blk[kPlanWarps + 1];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const bool lead = blockIdx.x == 0;
+  allow_next_launch();
+  wait_for_inputs();
 
   const int per = (a.batch + kPlanThreads - 1) / kPlanThreads;
   const int b0 = min(tid * per, a.batch), b1 = min(b0 + per, a.batch);
@@ -342,6 +344,8 @@ __global__ void __launch_bounds__(2 * kThreads, kThreads == 128 ? 3 : 16) append
   const int g = blockIdx.y;
   const int is_v = threadIdx.x / kThreads;
   const int64_t item = blockIdx.x;
+  allow_next_launch();
+  wait_for_inputs();
   const BlockRows rows = find_block(a, item, lane);
   if (rows.state != BlockRows::kFound) {
     // lengths that disagree with the packed rows: nothing is written
@@ -439,8 +443,7 @@ cudaError_t launch_plan(const PlanArgs& args, cudaStream_t stream) {
   }
   const int64_t per = kTokens * kPlanThreads, want = (args.total_new + per - 1) / per;
   const unsigned grid = static_cast<unsigned>(want < 1 ? 1 : want > 148 * 4 ? 148 * 4 : want);
-  plan_pages_kernel<kTokens><<<grid, kPlanThreads, smem, stream>>>(args);
-  return cudaGetLastError();
+  return launch_early(plan_pages_kernel<kTokens>, dim3(grid), dim3(kPlanThreads), smem, stream, args);
 }
 
 cudaError_t launch_plan_pages(const PlanArgs& args, cudaStream_t stream) {
@@ -456,11 +459,9 @@ cudaError_t launch_append_kv(const AppendArgs& args, cudaStream_t stream) {
   if (blocks == 0) return cudaSuccess;
   const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(args.num_groups));
   // Up to two tokens a request on average: single warps.
-  if (args.total_new <= 2 * static_cast<int64_t>(args.batch))
-    append_kv_kernel<32><<<grid, 64, 0, stream>>>(args);
-  else
-    append_kv_kernel<128><<<grid, 256, 0, stream>>>(args);
-  return cudaGetLastError();
+  return args.total_new <= 2 * static_cast<int64_t>(args.batch)
+             ? launch_early(append_kv_kernel<32>, grid, dim3(64), 0, stream, args)
+             : launch_early(append_kv_kernel<128>, grid, dim3(256), 0, stream, args);
 }
 
 }  // namespace ls
