@@ -10,6 +10,7 @@ from ._native import LeanSelectError, LS_MAX_TOPK, version
 from .attention import (CompressK, LayerConfig, infllmv2_attn_varlen_func,
                         lightweight_compressed_attention, nosa_atom_scores,
                         prefill_layer_attention)
+from .kvcache import PagedKVCache
 from .selector import LeanSelectSelector
 from .uniform import uniform_prefill_topk_idx
 
@@ -17,5 +18,5 @@ __all__ = [
     "ops", "LeanSelectError", "LS_MAX_TOPK", "version", "CompressK", "LayerConfig",
     "infllmv2_attn_varlen_func", "lightweight_compressed_attention", "nosa_atom_scores",
     "prefill_layer_attention",
-    "LeanSelectSelector", "uniform_prefill_topk_idx",
+    "LeanSelectSelector", "PagedKVCache", "uniform_prefill_topk_idx",
 ]

@@ -19,12 +19,14 @@ from __future__ import annotations
 
 import math
 from dataclasses import dataclass, field
-from typing import Sequence
+from typing import Callable, Sequence
 
 import torch
 
 from . import host_kernels as hk
+from . import ops
 from .attention import LayerConfig, count_attended_keys, prefill_layer_attention
+from .kvcache import PagedKVCache
 from .selector import LeanSelectSelector
 
 
@@ -189,23 +191,36 @@ class PrefillModel:
 
     def prefill(self, input_ids: torch.Tensor, cu_seqlens: torch.Tensor,
                 lengths: Sequence[int], timers: list | None = None,
-                key_counts: list | None = None, capture: dict | None = None) -> torch.Tensor:
+                key_counts: list | None = None, capture: dict | None = None,
+                cache: PagedKVCache | None = None) -> torch.Tensor:
         """Packed prefill of ``len(lengths)`` sequences; returns ``[B, vocab]`` fp32 logits.
 
         ``timers`` (optional) collects per-layer hot-path stage events (see
         ``prefill_layer_attention``); ``key_counts`` (optional, adds host
         syncs) collects each layer's attended-key count; ``capture``
         (optional dict) receives the last layer's attention inputs
-        (``q``, ``k``, ``v``, ``idx``, ``cu``, ``max_len``) for profiling.
+        (``q``, ``k``, ``v``, ``idx``, ``cu``, ``max_len``) for profiling;
+        ``cache`` (optional, empty) keeps every layer's keys and values in 8
+        bits for :meth:`decode`.
         """
         s = self.shape
         lengths = [int(n) for n in lengths]
-        positions = torch.cat([torch.arange(n, device=self.device) for n in lengths])
+        plan = None
+        if cache is not None:
+            if cache.max_seqlen:
+                raise ValueError("prefill fills an empty cache")
+            plan = cache.plan(lengths)
+            # The frequencies its keys are rotated by; decode keeps to them.
+            cache.rope_len = max(lengths)
+        positions = (plan.positions if plan is not None else
+                     torch.cat([torch.arange(n, device=self.device) for n in lengths]))
         freqs = self.rope.frequencies(max(lengths))
         h = self.embed[input_ids] * s.scale_emb
         max_len = max(lengths)
-        for layer in self.layers:
+        for i, layer in enumerate(self.layers):
             q, k, v = self.qkv(layer, h, positions, freqs)
+            if plan is not None:
+                ops.append_kv(k, v, plan, *cache.layer(i))
             attn, idx = prefill_layer_attention(q, k, v, cu_seqlens, max_len, layer.selector,
                                                 s.sparse, lengths=lengths, return_topk=True,
                                                 timers=timers)
@@ -219,3 +234,35 @@ class PrefillModel:
             self.mlp_residual(layer, h)
         last = cu_seqlens[1:].long() - 1
         return self.logits(h[last])
+
+    # -- decode over the 8-bit cache ---------------------------------------------------
+
+    def decode(self, input_ids: torch.Tensor, cache: PagedKVCache,
+               new_lens: Sequence[int] | None = None,
+               page_lists: Callable[[int, torch.Tensor], torch.Tensor] | None = None
+               ) -> torch.Tensor:
+        """One step after :meth:`prefill`: logits ``[total, vocab]`` of every new token.
+
+        ``input_ids`` holds the new tokens packed by request, one each unless
+        ``new_lens`` says otherwise (a draft of several tokens is scored in one
+        step).  Attention runs over all cached pages, or over those that
+        ``page_lists(layer, q)`` returns as ``[G, total, T]`` block numbers.
+        """
+        s = self.shape
+        new = [1] * cache.batch if new_lens is None else [int(n) for n in new_lens]
+        if sum(new) != input_ids.numel():
+            raise ValueError("input_ids must hold sum(new_lens) tokens")
+        if not cache.max_seqlen:
+            raise ValueError("decode continues a cache that prefill has filled")
+        plan = cache.plan(new)
+        freqs = self.rope.frequencies(cache.rope_len)
+        h = self.embed[input_ids] * s.scale_emb
+        for i, layer in enumerate(self.layers):
+            q, k, v = self.qkv(layer, h, plan.positions, freqs)
+            ops.append_kv(k, v, plan, *cache.layer(i))
+            lists = page_lists(i, q) if page_lists is not None else None
+            attn = ops.paged_attn(q, *cache.layer(i), cache.block_table, plan.seq_lens,
+                                  plan.cu_seqlens_q, max(new), cache.max_seqlen, topk_idx=lists)
+            h.addmm_(attn.view(h.shape[0], -1), layer.w_o.t(), alpha=self.residual_scale)
+            self.mlp_residual(layer, h)
+        return self.logits(h)

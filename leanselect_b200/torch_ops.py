@@ -95,6 +95,62 @@ def _(q, k, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, topk_idx,
     return (torch.empty_like(q), q.new_empty((q.shape[1], q.shape[0]), dtype=torch.float32))
 
 
-OPS = ("compress_keys", "project_atom_keys", "select_pages", "score_pages", "sparse_attn")
+@torch.library.custom_op("leanselect_b200::plan_pages", mutates_args=("block_table",))
+def plan_pages(context_lens: Tensor, new_lens: Tensor, block_table: Tensor, free_pages: Tensor,
+               free_head: Tensor, total_new: int
+               ) -> tuple[Tensor, Tensor, Tensor, Tensor, Tensor, Tensor]:
+    """``(seq_lens, cu_seqlens_q, cu_blocks, slots, positions, free_head)`` of one step."""
+    p = ops.plan_pages(context_lens, new_lens, block_table, free_pages, free_head, total_new)
+    # A custom op's results share no storage; the plan's vectors are slices of one buffer.
+    return tuple(t.clone() for t in (p.seq_lens, p.cu_seqlens_q, p.cu_blocks, p.slots, p.positions,
+                                     p.free_head))
+
+
+@plan_pages.register_fake
+def _(context_lens, new_lens, block_table, free_pages, free_head, total_new):
+    batch = context_lens.shape[0]
+
+    def vec(n, dtype=torch.int32):
+        return context_lens.new_empty((n,), dtype=dtype)
+
+    return (vec(batch), vec(batch + 1), vec(batch + 1), vec(total_new, torch.int64),
+            vec(total_new, torch.int64), vec(1))
+
+
+@torch.library.custom_op("leanselect_b200::append_kv",
+                         mutates_args=("k_pages", "v_pages", "k_scale", "v_scale"))
+def append_kv(k: Tensor, v: Tensor, context_lens: Tensor, seq_lens: Tensor, cu_seqlens_q: Tensor,
+              cu_blocks: Tensor, slots: Tensor, k_pages: Tensor, v_pages: Tensor, k_scale: Tensor,
+              v_scale: Tensor) -> None:
+    """Round a planned step's keys and values into the 8-bit pages."""
+    plan = ops.PagePlan(context_lens, seq_lens, cu_seqlens_q, cu_blocks, slots, None)
+    ops.append_kv(k, v, plan, k_pages, v_pages, k_scale, v_scale)
+
+
+@append_kv.register_fake
+def _(k, v, context_lens, seq_lens, cu_seqlens_q, cu_blocks, slots, k_pages, v_pages, k_scale,
+      v_scale):
+    return None
+
+
+@torch.library.custom_op("leanselect_b200::paged_attn", mutates_args=())
+def paged_attn(q: Tensor, k_pages: Tensor, v_pages: Tensor, k_scale: Tensor, v_scale: Tensor,
+               block_table: Tensor, seq_lens: Tensor, cu_seqlens_q: Tensor, max_seqlen_q: int,
+               max_seqlen_k: int, topk_idx: Tensor | None, softmax_scale: float,
+               causal: bool) -> tuple[Tensor, Tensor]:
+    """Attention over the 8-bit paged cache: ``(out, lse)``; ``softmax_scale`` 0: ``D**-0.5``."""
+    return ops.paged_attn(q, k_pages, v_pages, k_scale, v_scale, block_table, seq_lens,
+                          cu_seqlens_q, max_seqlen_q, max_seqlen_k, topk_idx=topk_idx,
+                          softmax_scale=softmax_scale or None, causal=causal, return_lse=True)
+
+
+@paged_attn.register_fake
+def _(q, k_pages, v_pages, k_scale, v_scale, block_table, seq_lens, cu_seqlens_q, max_seqlen_q,
+      max_seqlen_k, topk_idx, softmax_scale, causal):
+    return (torch.empty_like(q), q.new_empty((q.shape[1], q.shape[0]), dtype=torch.float32))
+
+
+OPS = ("compress_keys", "project_atom_keys", "select_pages", "score_pages", "sparse_attn",
+       "plan_pages", "append_kv", "paged_attn")
 
 __all__ = list(OPS)

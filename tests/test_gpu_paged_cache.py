@@ -583,3 +583,240 @@ def test_prompt_then_decode_steps():
         assert bool(((got.double().cpu() - want).abs() <= tol).all())
         context, at = ref["seq"], ref["head"]
         ctx, head = plan.seq_lens, plan.free_head
+
+
+# ---------------------------------------------------------------------------
+# streams, graphs, custom ops
+# ---------------------------------------------------------------------------
+
+def step_inputs(batch, G, H, seed, length):
+    """Device tensors of a decode step over a filled cache."""
+    gen = torch.Generator().manual_seed(seed)
+    seq = torch.randint(1, length + 1, (batch,), generator=gen).tolist()
+    codes, scales, table = make_cache([n + 8 for n in seq], G, seed, nan_tail=False)
+    cache = [codes[0].to(DEV), codes[1].to(DEV), scales[0].to(DEV), scales[1].to(DEV)]
+    q = torch.randn(batch, H, 128, generator=gen).bfloat16().to(DEV)
+    return seq, cache, i32(table), q
+
+
+def test_calls_on_several_streams_at_once():
+    """Interleaved steps of four batches on four streams give what each gives alone."""
+    steps = [step_inputs(b, 2, 32, b, 3000) for b in (1, 7, 64, 3)]
+    args = [(q, *cache, table, i32(seq), i32(list(range(len(seq) + 1))), 1, max(seq))
+            for seq, cache, table, q in steps]
+    alone = [ops.paged_attn(*a) for a in args]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in args]
+    got = [[] for _ in args]
+    for _ in range(6):
+        for i, (s, a) in enumerate(zip(streams, args)):
+            with torch.cuda.stream(s):
+                got[i].append(ops.paged_attn(*a))
+    torch.cuda.synchronize()
+    for i, outs in enumerate(got):
+        assert all(torch.equal(o, alone[i]) for o in outs)
+
+
+def test_two_captured_steps_replayed_together():
+    """Graphs of a whole decode step (plan, write, attention) advance on the device;
+    two of them replayed on two streams equal the eager steps."""
+    G, H, steps = 2, 16, 5
+
+    def state(batch, seed):
+        seq, cache, table, _ = step_inputs(batch, G, H, seed, 200)
+        width = table.shape[1]
+        more = torch.full((batch, 3), -1, dtype=torch.int32, device=DEV)
+        pool = cache[0].shape[0]
+        grown = [torch.cat([c, c[:batch]]).clone() if c.dtype != FP8 else
+                 torch.cat([c.view(torch.uint8), c.view(torch.uint8)[:batch]]).view(FP8).clone()
+                 for c in cache]
+        # the make_cache tables already hold room for eight more tokens
+        gen = torch.Generator().manual_seed(seed)
+        feed = [(torch.randn(batch, G, 128, generator=gen).bfloat16().to(DEV),
+                 torch.randn(batch, G, 128, generator=gen).bfloat16().to(DEV),
+                 torch.randn(batch, H, 128, generator=gen).bfloat16().to(DEV))
+                for _ in range(steps)]
+        table = torch.cat([table, more], dim=1)
+        for b, n in enumerate(seq):  # blocks past the cached tokens are handed out again
+            table[b, up(n):] = -1
+        return dict(ctx=i32(seq), cache=grown, table=table.contiguous(), width=width,
+                    free=torch.arange(pool, pool + batch, dtype=torch.int32, device=DEV),
+                    head=i32([0]), feed=feed, batch=batch, ones=i32([1] * batch))
+
+    def step(s, k, v, q):
+        plan = ops.plan_pages(s["ctx"], s["ones"], s["table"], s["free"], s["head"], s["batch"])
+        ops.append_kv(k, v, plan, *s["cache"])
+        out = ops.paged_attn(q, *s["cache"], s["table"], plan.seq_lens, plan.cu_seqlens_q, 1, 256)
+        s["ctx"].copy_(plan.seq_lens)
+        s["head"].copy_(plan.free_head)
+        return out
+
+    eager = []
+    for batch, seed in ((5, 1), (9, 2)):
+        s = state(batch, seed)
+        eager.append([step(s, *f).clone() for f in s["feed"]])
+        eager[-1].append([c.clone() for c in s["cache"]])
+    captured = []
+    for batch, seed in ((5, 1), (9, 2)):
+        s = state(batch, seed)
+        warm = state(batch, seed)
+        step(warm, *warm["feed"][0])
+        feed = [t.clone() for t in s["feed"][0]]
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step(s, *feed)
+        captured.append((s, feed, graph, out, torch.cuda.Stream(), []))
+    torch.cuda.synchronize()
+    for t in range(steps):
+        for s, feed, graph, out, stream, outs in captured:
+            with torch.cuda.stream(stream):
+                for dst, src in zip(feed, s["feed"][t]):
+                    dst.copy_(src)
+                graph.replay()
+                outs.append(out.clone())
+    torch.cuda.synchronize()
+    for want, (s, _, _, _, _, outs) in zip(eager, captured):
+        assert all(torch.equal(a, b) for a, b in zip(want[:-1], outs))
+        assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+                   for a, b in zip(want[-1], s["cache"]))
+
+
+def test_custom_ops_run_the_same_kernels():
+    import leanselect_b200.torch_ops  # noqa: F401
+
+    registered = torch.ops.leanselect_b200
+    seq, cache, table, q = step_inputs(4, 2, 16, 3, 500)
+    cu = i32([0, 1, 2, 3, 4])
+    want, want_lse = ops.paged_attn(q, *cache, table, i32(seq), cu, 1, max(seq), return_lse=True)
+    out, lse = registered.paged_attn(q, *cache, table, i32(seq), cu, 1, max(seq), None, 0.0, True)
+    assert torch.equal(out, want) and torch.equal(lse, want_lse)
+    tables = [table.clone(), table.clone()]
+    free = i32(list(range(10)))
+    plan = ops.plan_pages(i32(seq), i32([1, 0, 2, 1]), tables[0], free, i32([1]), 4)
+    got = registered.plan_pages(i32(seq), i32([1, 0, 2, 1]), tables[1], free, i32([1]), 4)
+    for a, b in zip(got, (plan.seq_lens, plan.cu_seqlens_q, plan.cu_blocks, plan.slots,
+                          plan.positions, plan.free_head)):
+        assert torch.equal(a, b)
+    assert torch.equal(*tables)
+    k = torch.randn(4, 2, 128, device=DEV).bfloat16()
+    twins = [[c.clone() for c in cache] for _ in range(2)]
+    ops.append_kv(k, k, plan, *twins[0])
+    registered.append_kv(k, k, plan.context_lens, *got[:4], *twins[1])
+    assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(*twins))
+
+
+# ---------------------------------------------------------------------------
+# the host model
+# ---------------------------------------------------------------------------
+
+@pytest.fixture(scope="module")
+def model():
+    from leanselect_b200.model import MiniCPMShape, PrefillModel
+
+    shape = MiniCPMShape(vocab_size=500, hidden_size=256, intermediate_size=512, num_layers=2,
+                         num_heads=16, num_kv_heads=2, max_position=4096,
+                         original_max_position=4096, router_heads=4, router_dim=32)
+    return PrefillModel(shape, DEV, seed=3)
+
+
+def test_model_decodes_over_its_cache(model, monkeypatch):
+    """Prefill with a cache, a draft of several tokens and single steps: each layer's
+    write and attention equal the oracle's on the tensors the model gave them."""
+    from leanselect_b200 import PagedKVCache
+
+    s = model.shape
+    lengths = [150, 64, 5]
+    gen = torch.Generator().manual_seed(1)
+    ids = torch.randint(0, s.vocab_size, (sum(lengths),), generator=gen).to(DEV)
+    cu = i32(prefix(lengths))
+    cache = PagedKVCache(s.num_layers, 3, 200, 12, s.num_kv_heads, device=DEV)
+    plain = model.prefill(ids, cu, lengths)
+    assert torch.equal(model.prefill(ids, cu, lengths, cache=cache), plain)
+    assert cache.lengths == lengths and cache.seq_lens.tolist() == lengths
+
+    calls = []
+    append, attend = ops.append_kv, ops.paged_attn
+
+    def spy_append(k, v, plan, *layer):
+        before = [as_values(layer[0]), as_values(layer[1]), layer[2].double().cpu(),
+                  layer[3].double().cpu()]
+        append(k, v, plan, *layer)
+        context, new = plan.context_lens.tolist(), torch.diff(plan.cu_seqlens_q).tolist()
+        table = cache.block_table.tolist()
+        ora.append(k.cpu(), context, new, table, before[0], before[2])
+        ora.append(v.cpu(), context, new, table, before[1], before[3])
+        for got, want in zip((as_values(layer[0]), as_values(layer[1]), layer[2].double().cpu(),
+                              layer[3].double().cpu()), before):
+            assert torch.equal(got.nan_to_num(0), want.nan_to_num(0))
+        calls.append("write")
+
+    def spy_attend(q, *args, **kwargs):
+        out = attend(q, *args, **kwargs)
+        kp, vp, ks, vs, table, seq, cuq = args[:7]
+        idx = kwargs.get("topk_idx")
+        want, _, bounds = ora.attend(q.cpu(), as_values(kp), as_values(vp), ks.cpu(), vs.cpu(),
+                                     table.tolist(), seq.tolist(), cuq.tolist(),
+                                     None if idx is None else idx.cpu())
+        assert bool(((out.double().cpu() - want).abs() <= tolerance(want, bounds, 256)).all())
+        calls.append("attend")
+        return out
+
+    monkeypatch.setattr(ops, "append_kv", spy_append)
+    monkeypatch.setattr(ops, "paged_attn", spy_attend)
+    new = [3, 1, 0]
+    draft = torch.randint(0, s.vocab_size, (4,), generator=gen).to(DEV)
+    logits = model.decode(draft, cache, new)
+    assert logits.shape == (4, s.vocab_size) and bool(torch.isfinite(logits).all())
+    # one token each, over listed pages: the sink and the last pages
+    lists = torch.tensor([[[0, 1, 2], [0, 1, -1], [0, -1, -1]]] * 2, dtype=torch.int32, device=DEV)
+    logits = model.decode(draft[:3], cache, page_lists=lambda i, q: lists)
+    assert logits.shape == (3, s.vocab_size)
+    assert cache.lengths == [154, 66, 6] and cache.seq_lens.tolist() == [154, 66, 6]
+    assert calls == ["write", "attend"] * (2 * s.num_layers)
+    # A finished request's pages serve the next one.
+    cache.release(1)
+    assert cache.taken == 3 + 1 and cache.seq_lens.tolist() == [154, 0, 6]
+    model.decode(torch.zeros(40, dtype=torch.long, device=DEV), cache, [0, 40, 0])
+    assert cache.block_table[1, 0].item() >= 0 and cache.taken == 5
+
+
+def test_generate_is_the_loop_of_its_steps(model):
+    from leanselect_b200 import PagedKVCache
+    from leanselect_b200.runner import PrefillRunner
+
+    runner = PrefillRunner(model.shape, DEV, model=model)
+    lengths, steps = [70, 3], 4
+    gen = torch.Generator().manual_seed(2)
+    ids = torch.randint(0, model.shape.vocab_size, (sum(lengths),), generator=gen)
+    out = runner.generate(ids, lengths, steps)
+    assert out.shape == (2, steps) and out.device.type == "cpu"
+    cache = PagedKVCache(model.shape.num_layers, 2, 80, 4, 2, device=DEV)
+    tok = model.prefill(ids.to(DEV), i32(prefix(lengths)), lengths, cache=cache).argmax(-1)
+    for t in range(steps):
+        assert torch.equal(tok.cpu(), out[:, t])
+        if t + 1 < steps:
+            tok = model.decode(tok, cache).argmax(-1)
+    for bad in (([], 3), ([0, 5], 3), (lengths, 0)):
+        with pytest.raises(ValueError):
+            runner.generate(ids, *bad)
+
+
+def test_model_decode_refusals(model):
+    from leanselect_b200 import PagedKVCache
+
+    s = model.shape
+    cache = PagedKVCache(s.num_layers, 1, 65, 1, s.num_kv_heads, device=DEV)
+    with pytest.raises(ValueError, match="prefill"):
+        model.decode(torch.zeros(1, dtype=torch.long, device=DEV), cache)
+    ids = torch.zeros(64, dtype=torch.long, device=DEV)
+    model.prefill(ids, i32([0, 64]), [64], cache=cache)
+    with pytest.raises(ValueError, match="empty"):
+        model.prefill(ids, i32([0, 64]), [64], cache=cache)
+    with pytest.raises(ValueError, match="sum"):
+        model.decode(ids[:2], cache)
+    with pytest.raises(ValueError, match="tokens"):
+        model.decode(ids[:2], cache, [2])
+    with pytest.raises(RuntimeError, match="out of pages"):
+        model.decode(ids[:1], cache)
+    assert cache.lengths == [64] and cache.taken == 1

@@ -142,3 +142,43 @@ def test_oracle_attention_is_softmax_over_the_listed_keys():
     ref = torch.nn.functional.scaled_dot_product_attention(q[0].double(), kk, vv)
     assert torch.allclose(out[0], ref, atol=1e-12)
     assert torch.allclose(lse[:, 0], torch.logsumexp(q[0].double() @ kk.T / 128 ** 0.5, -1))
+
+
+def test_cache_refuses_on_the_host():
+    """Bookkeeping errors are raised before anything is launched."""
+    from leanselect_b200 import PagedKVCache
+
+    for bad in (dict(batch=0), dict(num_layers=0), dict(num_pages=0), dict(head_dim=64),
+                dict(batch=_native.LS_MAX_PLAN_BATCH + 1), dict(max_tokens=0)):
+        with pytest.raises(ValueError):
+            PagedKVCache(**{**dict(num_layers=1, batch=2, max_tokens=100, num_pages=3,
+                                   num_kv_heads=1, device="cpu"), **bad})
+    cache = PagedKVCache(1, 2, 100, 3, 1, device="cpu")
+    assert cache.block_table.shape == (2, 2) and cache.max_seqlen == 0
+    for new in ([1], [1, -1], [101, 0]):
+        with pytest.raises(ValueError):
+            cache.plan(new)
+    with pytest.raises(RuntimeError, match="out of pages"):
+        cache.plan([100, 70])
+    assert cache.lengths == [0, 0] and cache.taken == 0
+
+
+def test_custom_op_shapes():
+    import leanselect_b200.torch_ops  # noqa: F401
+
+    def t(*shape, dtype=torch.int32):
+        return torch.empty(shape, dtype=dtype, device="meta")
+
+    registered = torch.ops.leanselect_b200
+    fp8 = torch.float8_e4m3fn
+    seq, cu_q, cu_blocks, slots, pos, head = registered.plan_pages(t(5), t(5), t(5, 9), t(30), t(1),
+                                                                   70)
+    assert (seq.shape, cu_q.shape, cu_blocks.shape, head.shape) == ((5,), (6,), (6,), (1,))
+    assert slots.shape == pos.shape == (70,) and slots.dtype == pos.dtype == torch.int64
+    cache = (t(8, 2, 64, 128, dtype=fp8), t(8, 2, 64, 128, dtype=fp8),
+             t(8, 2, dtype=torch.float32), t(8, 2, dtype=torch.float32))
+    kv = t(70, 2, 128, dtype=torch.bfloat16)
+    assert registered.append_kv(kv, kv, t(5), seq, cu_q, cu_blocks, slots, *cache) is None
+    out, lse = registered.paged_attn(t(70, 16, 128, dtype=torch.bfloat16), *cache, t(5, 9), seq,
+                                     cu_q, 30, 500, None, 0.0, True)
+    assert out.shape == (70, 16, 128) and lse.shape == (16, 70) and lse.dtype == torch.float32
