@@ -46,7 +46,7 @@ constexpr int kProducerRegs = 72, kConsumerRegs = 216, kLaunchRegs = 168;
 static_assert(kProducerRegs + kTeams * kConsumerRegs <= (kTeams + 1) * kLaunchRegs,
               "the split must fit the registers the block is launched with");
 static_assert(kTeams * kPairs == 4, "warpgroup 0 has one producer warp per pair");
-constexpr int kMinUnits = 2;                 // pages a range has at least
+constexpr int kMinUnits = 1;                 // pages a range has at least
 constexpr int kRingBytes = kStages * kStageBytes;
 constexpr int kSumBytes = kWarps * 16 * 128 * 4;  // a team's row sums, one set per warp
 constexpr float kSlack = 14.f, kHeadroom = 6.f;  // binades, see above
@@ -345,6 +345,27 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
       const int row = w0 / args.topk;
       shared->team[threadIdx.x].start = {-1, row / rows_listed, row % rows_listed,
                                          w0 - row * args.topk};
+    }
+  } else if (args.batch <= 32) {
+    // One request per lane, in every warp: no meeting of the block.
+    Request r{0, 0, 0, false};
+    if (lane < args.batch) r = load_request(args, lane);
+    if (r.bad && blockIdx.x == 0 && warp_id == 0) report(args.status, LS_DEVERR_SEQLENS);
+    const int pages = scheduled_pages(r.len), own = r.nq * G * pages;
+    int upto = own;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += y;
+    }
+    work = __shfl_sync(0xffffffffu, upto, 31);
+    const Cut cut(work);
+    if (warp_id < kTeams) {
+      const int off = range0 + warp_id < cut.ranges ? cut.start(range0 + warp_id) - (upto - own) : -1;
+      if (off >= 0 && off < own) {
+        const int row = off / pages;
+        shared->team[warp_id].start = {lane, row / r.nq, row % r.nq, off - row * pages};
+      }
     }
   } else {
     const int per = (args.batch + kThreads - 1) / kThreads;
@@ -851,6 +872,15 @@ size_t paged_smem_bytes() {
   return 1024 + kTeams * (kPairs * kRingBytes + kSumBytes) + sizeof(PagedSmem);
 }
 
+// A load that stays where it is written, ahead of the sums that use it.
+__device__ __forceinline__ float4 load_part(const float* p) {
+  float4 x;
+  asm volatile("ld.global.cg.v4.f32 {%0,%1,%2,%3}, [%4];"
+               : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w)
+               : "l"(p));
+  return x;
+}
+
 // Writes one joined row of one head: lane l holds its dims 4l .. 4l + 3.
 __device__ __forceinline__ void write_row(const PagedAttnArgs& args, int row, int head, int lane,
                                           float4 o, float m, float l) {
@@ -875,8 +905,11 @@ __device__ __forceinline__ int64_t part_row(int j, int i, int head) {
 }
 
 // Far fewer rows than ranges (a decode step of a few long requests): a row has
-// many parts.  One block per (row, head); warp w sums parts w, w + 16, ...
-constexpr int kMergeWarps = 16;
+// many parts.  One block per (row, head); thread k looks after range k, warp w
+// sums parts w, w + 24, ...  What a range's parts weigh is loaded with its
+// header, before it is known which of them belong to the row: the kernel is a
+// chain of round trips, and this one saves a link.
+constexpr int kMergeWarps = 24, kMergeAhead = 7;
 
 __global__ void __launch_bounds__(32 * kMergeWarps) paged_merge_many_kernel(
     const __grid_constant__ PagedAttnArgs args, int ranges) {
@@ -891,7 +924,14 @@ __global__ void __launch_bounds__(32 * kMergeWarps) paged_merge_many_kernel(
   __syncthreads();
   allow_next_launch();
   wait_for_inputs();
-  const int2 head = tid < ranges ? args.headers[tid] : make_int2(-1, 1);
+  const float2* mls = reinterpret_cast<const float2*>(args.part_ml);
+  int2 head = make_int2(-1, 1);
+  float2 ml = make_float2(-INFINITY, 0.f), begin = ml;
+  if (tid < ranges) {
+    head = args.headers[tid];
+    ml = mls[static_cast<int64_t>(2 * tid) * 16 + h];
+    begin = mls[static_cast<int64_t>(2 * tid + 1) * 16 + h];
+  }
   if (head.x == row) first = tid;
   __syncthreads();
   const int j = first;
@@ -899,8 +939,8 @@ __global__ void __launch_bounds__(32 * kMergeWarps) paged_merge_many_kernel(
   if (tid > j && tid < ranges && head.y != 0) atomicMin(&behind, tid);
   __syncthreads();
   const int n = min(behind, ranges - 1) - j + 1;
-  const float2 ml = tid < n ? reinterpret_cast<const float2*>(args.part_ml)[part_row(j, tid, h)]
-                            : make_float2(-INFINITY, 0.f);
+  if (tid == j) ml = begin;
+  if (tid < j || tid >= j + n) ml = make_float2(-INFINITY, 0.f);
   float m = ml.x;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
@@ -909,21 +949,27 @@ __global__ void __launch_bounds__(32 * kMergeWarps) paged_merge_many_kernel(
 #pragma unroll
   for (int w = 0; w < kMergeWarps; ++w) m = fmaxf(m, warp_m[w]);
   const float mine = ml.x == -INFINITY ? 0.f : ex2(ml.x - m);
-  if (tid < n) weight[tid] = mine;
-  float l = ml.y * mine;
+  if (tid >= j && tid < j + n) weight[tid - j] = mine;
+  float l = ml.x == -INFINITY ? 0.f : ml.y * mine;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
   if (lane == 0) warp_l[warp] = l;
   __syncthreads();
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 10
-  for (int i = warp; i < n; i += kMergeWarps) {
-    const float w = weight[i];
-    const float4 x = reinterpret_cast<const float4*>(args.part_o + part_row(j, i, h) * 128)[lane];
-    acc.x = fmaf(x.x, w, acc.x);
-    acc.y = fmaf(x.y, w, acc.y);
-    acc.z = fmaf(x.z, w, acc.z);
-    acc.w = fmaf(x.w, w, acc.w);
+  for (int base = warp; base < n; base += kMergeAhead * kMergeWarps) {
+    float4 x[kMergeAhead];
+#pragma unroll
+    for (int k = 0; k < kMergeAhead; ++k) {
+      const int i = min(base + k * kMergeWarps, n - 1);  // no branch: all loads in flight
+      x[k] = load_part(args.part_o + part_row(j, i, h) * 128 + 4 * lane);
+    }
+#pragma unroll
+    for (int k = 0; k < kMergeAhead; ++k) {
+      const int i = base + k * kMergeWarps;
+      const float w = i < n ? weight[i] : 0.f;
+      acc = make_float4(fmaf(x[k].x, w, acc.x), fmaf(x[k].y, w, acc.y), fmaf(x[k].z, w, acc.z),
+                        fmaf(x[k].w, w, acc.w));
+    }
   }
   sum[warp][lane] = acc;
   __syncthreads();
@@ -950,35 +996,42 @@ __global__ void __launch_bounds__(256) paged_merge_few_kernel(
   wait_for_inputs();
   if (h >= args.heads_per_group) return;
   const int row = args.headers[j].x;
-  if (row < 0) return;
+  if (row < 0) return;  // most ranges here
   float m = -INFINITY, l = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   bool more = true;
   for (int base = 0; more; base += 32) {
     const int k = j + base + lane;
-    const uint32_t ends =
-        __ballot_sync(0xffffffffu, k >= ranges || (base + lane > 0 && args.headers[k].y != 0));
+    int ends_row = 1;
+    float2 ml = make_float2(-INFINITY, 0.f);
+    if (k < ranges) {
+      ends_row = args.headers[k].y;
+      ml = reinterpret_cast<const float2*>(args.part_ml)[part_row(j, base + lane, h)];
+    }
+    const uint32_t ends = __ballot_sync(0xffffffffu, base + lane > 0 && ends_row != 0);
     more = ends == 0;
-    int n = more ? 32 : __ffs(ends);
-    if (j + base + n > ranges) n = ranges - j - base;
-    const float2 ml = lane < n ? reinterpret_cast<const float2*>(
-                                     args.part_ml)[part_row(j, base + lane, h)]
-                               : make_float2(-INFINITY, 0.f);
+    const int n = min(more ? 32 : __ffs(ends), ranges - j - base);
+    if (lane >= n) ml.x = -INFINITY;
     float mx = fmaxf(m, ml.x);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
     const float keep = m == -INFINITY ? 0.f : ex2(m - mx);
     const float w = ml.x == -INFINITY ? 0.f : ex2(ml.x - mx);
     m = mx;
-    l = fmaf(l, keep, ml.y * w);  // a lane's share; summed at the end
+    l = fmaf(l, keep, ml.x == -INFINITY ? 0.f : ml.y * w);  // a lane's share; summed at the end
     acc = make_float4(acc.x * keep, acc.y * keep, acc.z * keep, acc.w * keep);
-#pragma unroll 4
-    for (int i = 0; i < n; ++i) {
-      const float wi = __shfl_sync(0xffffffffu, w, i);
-      const float4 x =
-          reinterpret_cast<const float4*>(args.part_o + part_row(j, base + i, h) * 128)[lane];
-      acc = make_float4(fmaf(x.x, wi, acc.x), fmaf(x.y, wi, acc.y), fmaf(x.z, wi, acc.z),
-                        fmaf(x.w, wi, acc.w));
+    for (int i = 0; i < n; i += 4) {
+      float4 x[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        x[u] = load_part(args.part_o + part_row(j, base + min(i + u, n - 1), h) * 128 + 4 * lane);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const float wi = __shfl_sync(0xffffffffu, w, (i + u) & 31);
+        const float f = i + u < n ? wi : 0.f;
+        acc = make_float4(fmaf(x[u].x, f, acc.x), fmaf(x[u].y, f, acc.y), fmaf(x[u].z, f, acc.z),
+                          fmaf(x[u].w, f, acc.w));
+      }
     }
   }
 #pragma unroll
