@@ -890,10 +890,19 @@ int ls_paged_attn(const uint16_t* q, const uint8_t* k_pages, const uint8_t* v_pa
   a.status = status;
   // At most one range per scheduled page: the caller's max_seqlen_k bounds the
   // pages of a dense row (a longer request only gets fewer ranges).
-  LS_REQUIRE(total_q * num_kv_heads * std::max<int64_t>(topk > 0 ? topk : max_blocks, 1) <
+  LS_REQUIRE(total_q * num_kv_heads * ((topk > 0 ? topk : max_blocks) + kPagedRowCost) <
                  (int64_t{1} << 31),
              "total_q * num_kv_heads * pages per row out of range");
-  const int64_t per_row = topk > 0 ? topk : std::max<int64_t>(1, (int64_t{max_seqlen_k} + 63) / 64);
+  const int64_t most_pages = std::max<int64_t>(1, (int64_t{max_seqlen_k} + 63) / 64);
+  a.units = static_cast<int>(topk > 0 ? std::min<int64_t>(topk, most_pages) : 0);
+  // A tile of 16 rows takes as many tokens of a request as their heads fit, so
+  // that a draft or a chunk reads each page once for all of them.  Their page
+  // lists are joined where a table of the request's pages fits on chip; on
+  // longer requests the lists share little.
+  a.pack = 1;
+  if (max_seqlen_q > 1 && (topk == 0 || most_pages <= kPagedMaxUnion))
+    a.pack = std::min(16 / hg, static_cast<int>(max_seqlen_q));
+  const int64_t per_row = topk > 0 ? a.units : most_pages;
   const int64_t want = total_q * num_kv_heads * per_row;
   const int ranges = static_cast<int>(std::min<int64_t>({want, 2 * sms, kPagedMaxRanges}));
   err = launch_paged_attn(a, ranges, static_cast<cudaStream_t>(stream));

@@ -192,6 +192,11 @@ cudaError_t launch_append_kv(const AppendArgs& args, cudaStream_t stream);
 // Attention over the paged cache (paged_attn.cu).
 constexpr int kPagedMaxRanges = 2 * 148;  // work ranges: two on each of the B200's SMs
 
+// Units of work a row counts for besides its pages.
+constexpr int kPagedRowCost = 4;
+// Most pages of a request whose tokens' page lists are joined in one tile.
+constexpr int kPagedMaxUnion = 512;
+
 struct PagedAttnArgs {
   CUtensorMap tm_k;       // K codes as [num_pages * G * 64, 128] bytes, box {128, 64}, 128B swizzle
   CUtensorMap tm_v;
@@ -210,11 +215,14 @@ struct PagedAttnArgs {
   int heads_per_group;    // 1 .. 16
   const int32_t* topk_idx;  // [G, total_q, topk], topk == 0: every page of the request
   int topk;
+  int units;              // lists of single tokens: pages a row is scheduled with
+  int pack;               // tokens of one request in a 16-row tile
   int causal;
   float scale_log2;       // softmax_scale * log2(e)
   uint16_t* out;
   float* lse;
-  int2* headers;          // workspace: per range, the row it leaves unfinished and that row's last range
+  int2* headers;          // workspace, per range: the row it leaves unfinished (-1: none);
+                          // that row's tokens << 1 | whether a row that comes in ends here
   float* part_ml;         // [2 * ranges, 16, 2]: row reference (log2) and row sum
   float* part_o;          // [2 * ranges, 16, 128]
   int32_t* status;

@@ -58,15 +58,18 @@ enum StageFlag { kFirst = 1, kLast = 2, kData = 4, kStop = 8 };
 struct __align__(16) PageDesc {
   int key0;        // position of the page's first key
   float k_scale, v_log2, v_inv;
-  int limit;       // last visible position (-1: none)
-  int token;
+  int limit;       // last position the tile's last token sees
+  int token;       // the tile's first token
   int row;         // StageFlag | group << 4 | (workspace part + 1) << 20, part -1: none
   int y;           // the page's first row in the tensor maps (-1: no data)
+  int tokens;      // tokens of the tile
+  uint32_t mask;   // those of them that list the page
 };
 constexpr int kDescs = 64;  // a batch of 32 never reaches the stages still in the ring
 
-// The work unit a range begins at: unit `unit` of row (token, group), dense:
-// of request `b`, token being its row in the request.
+// The work unit a range begins at: unit `unit` of row (token, group) of
+// request `b`, token being the tile's first, counted in the request; with page
+// lists of single tokens b is -1 and the token counted in the batch.
 struct Start {
   int b, group, token, unit;
 };
@@ -75,7 +78,9 @@ struct PairSmem {
   uint64_t full[kStages];
   uint64_t empty[kStages];
   PageDesc desc[kDescs];
-  int32_t pages[LS_MAX_TOPK];  // listed: the row's sorted pages
+  // listed: the row's sorted pages; for tiles of several tokens page << 16 |
+  // the tokens that list it
+  uint32_t pages[kPagedMaxUnion];
 };
 
 struct TeamSmem {
@@ -177,10 +182,12 @@ __device__ __forceinline__ float bf16_hi(uint32_t w) { return __uint_as_float(w 
 // the row's largest value is near 1: f16 then holds every value to 2^-25 of
 // the largest.  The 32 dims a quad lane holds of a key row (32c ..) are the
 // contraction's order: k-step kk takes dims 32c + 4kk .. + 3.  kHalf: at most
-// 8 heads, rows 8 .. 15 of the tile stay zero.
+// 8 rows of heads, rows 8 .. 15 of the tile stay zero.
 template <bool kHalf>
-__device__ __forceinline__ void load_query(const uint16_t* q, int gq, int heads, float scale_log2,
-                                           uint32_t (&qa)[8][4], float* f0, float* f1) {
+__device__ __forceinline__ void load_query(const PagedAttnArgs& args, int token, int group,
+                                           int tokens, int gq, int c, uint32_t (&qa)[8][4],
+                                           float* f0, float* f1) {
+  const int heads = args.heads_per_group;
 #pragma unroll
   for (int half = 0; half < 2; ++half) {
     const int h = gq + 8 * half;
@@ -189,11 +196,14 @@ __device__ __forceinline__ void load_query(const uint16_t* q, int gq, int heads,
       for (int kk = 0; kk < 8; ++kk) qa[kk][1] = qa[kk][3] = 0;
       break;
     }
-    const uint4* src = reinterpret_cast<const uint4*>(q + h * 128);
+    // Tile row h is head h % heads of token h / heads.
+    const int64_t row =
+        static_cast<int64_t>(token + h / heads) * args.num_heads + group * heads + h % heads;
+    const uint4* src = reinterpret_cast<const uint4*>(args.q + row * 128 + 32 * c);
     uint4 raw[4];
     float amax = 0.f;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) raw[k] = h < heads ? __ldg(src + k) : make_uint4(0, 0, 0, 0);
+    for (int k = 0; k < 4; ++k) raw[k] = h < heads * tokens ? __ldg(src + k) : make_uint4(0, 0, 0, 0);
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       const uint32_t w[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
@@ -207,7 +217,7 @@ __device__ __forceinline__ void load_query(const uint16_t* q, int gq, int heads,
     // scale.
     const int e = min(max(static_cast<int>(__float_as_uint(amax) >> 23) - 127, -60), 78);
     const float down = __int_as_float((127 - e) << 23);
-    const float factor = scale_log2 * __int_as_float((127 + e) << 23);
+    const float factor = args.scale_log2 * __int_as_float((127 + e) << 23);
     if (half == 0) *f0 = factor; else *f1 = factor;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
@@ -218,6 +228,53 @@ __device__ __forceinline__ void load_query(const uint16_t* q, int gq, int heads,
             pack_f16x2(bf16_lo(w[j]) * down, bf16_hi(w[j]) * down);
     }
   }
+}
+
+// Whether the first `rows` of a warp's 32 value rows hold a NaN code.
+__device__ __forceinline__ bool has_nan(uint32_t v, int rows, int lane) {
+  bool found = false;
+  for (int r = lane; r < rows; r += 32)
+    for (int i = 0; i < 8; ++i) {
+      const uint4 x = lds128(v + r * 128 + ((i ^ r) & 7) * 16);
+      const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) found = found || __vcmpeq4(w[j] & 0x7F7F7F7Fu, 0x7F7F7F7Fu) != 0;
+    }
+  return __any_sync(0xffffffffu, found);
+}
+
+// The pages that any of a tile's tokens lists, ascending, as page << 16 | the
+// tokens that do; returns how many.  One bit per (page, token) is collected in
+// `pages` by page number, then the list is compacted in place.
+__device__ __forceinline__ int union_pages(const PagedAttnArgs& args, uint32_t* pages, int token,
+                                           int tokens, int g, int n_pages, int limit, int lane) {
+  const int most = min(n_pages, kPagedMaxUnion);
+  for (int i = lane; i < most; i += 32) pages[i] = 0;
+  __syncwarp();
+  bool bad = n_pages > kPagedMaxUnion;
+  const int32_t* list = args.topk_idx + (static_cast<int64_t>(g) * args.total_q + token) * args.topk;
+  for (int t = 0; t < tokens; ++t) {
+    const int limit_t = args.causal ? limit - (tokens - 1 - t) : limit;
+#pragma unroll
+    for (int r = 0; r < LS_MAX_TOPK / 32; ++r) {
+      const int pos = 32 * r + lane;
+      const int32_t p = pos < args.topk ? __ldg(list + t * args.topk + pos) : -1;
+      bad = bad || p >= n_pages;
+      if (p >= 0 && p < most && p * kPage <= limit_t) atomicOr(pages + p, 1u << t);
+    }
+  }
+  if (bad) report(args.status, LS_DEVERR_PAGE_INDEX);
+  __syncwarp();
+  int n = 0;
+  for (int base = 0; base < most; base += 32) {
+    const int i = base + lane;
+    const uint32_t m = i < most ? pages[i] : 0;
+    const uint32_t some = __ballot_sync(0xffffffffu, m != 0);
+    if (m != 0) pages[n + __popc(some & ((1u << lane) - 1))] = static_cast<uint32_t>(i) << 16 | m;
+    n += __popc(some);
+    __syncwarp();
+  }
+  return n;
 }
 
 // B fragments of 16 keys' values in f16.  A quad lane's four keys (2c, 2c + 1,
@@ -271,6 +328,16 @@ __device__ __forceinline__ int scheduled_pages(int len) {
   return len > 0 ? (len + kPage - 1) / kPage : 1;
 }
 
+// Units of a row of such a request: its pages, or as many as the tile's tokens
+// can list between them.  kPagedRowCost is added to every row: its queries,
+// the meeting of its warps and its output take about as long as four pages, so
+// that a range of many short rows would last longer than one of a long row
+// (requests of 15623, 1 and 7622 tokens, 8 heads: 34 us without it).
+__device__ __forceinline__ int row_units(const PagedAttnArgs& a, int len) {
+  const int pages = scheduled_pages(len);
+  return a.topk > 0 ? min(a.pack * a.topk, pages) : pages;
+}
+
 // A request as the kernels see it: lengths that would leave the packed rows
 // or the block table are cut and reported.
 struct Request {
@@ -302,7 +369,7 @@ struct Cut {
   __device__ __forceinline__ int start(int i) const { return i * size + min(i, longer); }
 };
 
-template <bool kHalf>
+template <bool kHalf, bool kShared>
 __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_constant__ PagedAttnArgs args) {
   extern __shared__ __align__(16) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
@@ -315,7 +382,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
   const int warp_id = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   const int G = args.num_groups;
-  const bool listed = args.topk > 0;
+  const bool listed = args.topk > 0, single = listed && !kShared;
+  const int pack = kShared ? args.pack : 1;  // tokens of a tile
 
   if (threadIdx.x < kTeams) {
     TeamSmem* t = &shared->team[threadIdx.x];
@@ -332,26 +400,29 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
   wait_for_inputs();
 
   // ---- the work of all rows, and where the teams' ranges start
-  // listed: row r = (group, token) has `topk` units, ordered group-major.
-  // dense: request by request, (group, token) rows of scheduled_pages units.
+  // Page lists of single tokens: row (group, token) has `units` units, ordered
+  // group-major.  Otherwise request by request, (group, tile of tokens) rows of
+  // row_units units.
   const int range0 = static_cast<int>(blockIdx.x) * kTeams;
   int work, rows_listed = 0;
-  if (listed) {
+  if (single) {
     rows_listed = min(max(__ldg(args.cu_q + args.batch), 0), static_cast<int>(args.total_q));
-    work = rows_listed * G * args.topk;
+    const int units = args.units + kPagedRowCost;
+    work = rows_listed * G * units;
     const Cut cut(work);
     if (threadIdx.x < kTeams && range0 + static_cast<int>(threadIdx.x) < cut.ranges && work > 0) {
       const int w0 = cut.start(range0 + threadIdx.x);
-      const int row = w0 / args.topk;
+      const int row = w0 / units;
       shared->team[threadIdx.x].start = {-1, row / rows_listed, row % rows_listed,
-                                         w0 - row * args.topk};
+                                         w0 - row * units};
     }
   } else if (args.batch <= 32) {
     // One request per lane, in every warp: no meeting of the block.
     Request r{0, 0, 0, false};
     if (lane < args.batch) r = load_request(args, lane);
     if (r.bad && blockIdx.x == 0 && warp_id == 0) report(args.status, LS_DEVERR_SEQLENS);
-    const int pages = scheduled_pages(r.len), own = r.nq * G * pages;
+    const int tiles = (r.nq + pack - 1) / pack;
+    const int units = row_units(args, r.len) + kPagedRowCost, own = tiles * G * units;
     int upto = own;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -363,8 +434,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
     if (warp_id < kTeams) {
       const int off = range0 + warp_id < cut.ranges ? cut.start(range0 + warp_id) - (upto - own) : -1;
       if (off >= 0 && off < own) {
-        const int row = off / pages;
-        shared->team[warp_id].start = {lane, row / r.nq, row % r.nq, off - row * pages};
+        const int row = off / units;
+        shared->team[warp_id].start = {lane, row / tiles, row % tiles * pack, off - row * units};
       }
     }
   } else {
@@ -377,7 +448,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
 #pragma unroll 1
     for (int b = b0; b < b1; ++b) {
       r = load_request(args, b);
-      own += r.nq * G * scheduled_pages(r.len);
+      own += (r.nq + pack - 1) / pack * G * (row_units(args, r.len) + kPagedRowCost);
       bad = bad || r.bad;
     }
     if (bad && blockIdx.x == 0) report(args.status, LS_DEVERR_SEQLENS);
@@ -404,13 +475,14 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
       if (off < 0 || off >= own) continue;
       for (int b = b0; b < b1; ++b) {
         if (b1 - b0 > 1) r = load_request(args, b);
-        const int pages = scheduled_pages(r.len), units = r.nq * G * pages;
-        if (off < units) {
-          const int row = off / pages;
-          shared->team[t].start = {b, row / r.nq, row % r.nq, off - row * pages};
+        const int tiles = (r.nq + pack - 1) / pack;
+        const int units = row_units(args, r.len) + kPagedRowCost, all = tiles * G * units;
+        if (off < all) {
+          const int row = off / units;
+          shared->team[t].start = {b, row / tiles, row % tiles * pack, off - row * units};
           break;
         }
-        off -= units;
+        off -= all;
       }
     }
   }
@@ -449,11 +521,19 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
     int2 head = make_int2(-1, 1);
     Start at = sm->start;
     Request req{0, 0, 0, false};
-    if (!listed) req = load_request(args, at.b);
+    if (!single) req = load_request(args, at.b);
+    // A border inside a row's leading units, which stand for its own cost, moves
+    // to the row's begin, here and below; `at.unit` counts pages from here on.
+    if (at.unit <= kPagedRowCost) {
+      left += at.unit;
+      at.unit = 0;
+    } else {
+      at.unit -= kPagedRowCost;
+    }
     while (left > 0 && ok) {
       // ---- the row that the next unit belongs to
-      int token;
-      if (listed) {
+      int token, tokens = 1;
+      if (single) {
         token = at.token;
         if (at.b < 0 || token < req.q0 || token >= req.q0 + req.nq) {
           at.b = find_sequence(args.cu_q, args.batch, token);
@@ -462,12 +542,15 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
         }
       } else {
         token = req.q0 + at.token;
+        tokens = min(pack, req.nq - at.token);
       }
-      const int units = listed ? args.topk : scheduled_pages(req.len);
-      const int unit_end = min(units, at.unit + left);
+      const int units = single ? args.units : row_units(args, req.len);
+      const int done = at.unit > 0 ? at.unit + kPagedRowCost : 0;
+      if (done + left <= kPagedRowCost) break;  // the row is the next range's
+      const int unit_end = min(units, done + left - kPagedRowCost);
       const int t_rel = token - req.q0;
       int limit = req.len - 1;
-      if (args.causal) limit = min(limit, req.len - req.nq + t_rel);
+      if (args.causal) limit = min(limit, req.len - req.nq + t_rel + tokens - 1);
       if (t_rel < 0 || t_rel >= req.nq) limit = -1;
       const int g = at.group;
       // A row cut by the range's borders goes to the workspace: its begin to
@@ -475,19 +558,20 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
       int part = -1;
       if (at.unit > 0) {
         part = 2 * range;
-        if (unit_end < units) head.y = 0;  // and goes on behind this range too
+        if (unit_end < units) head.y &= ~1;  // and goes on behind this range too
       } else if (unit_end < units) {
         part = 2 * range + 1;
         head.x = token * G + g;
+        head.y |= tokens << 1;
       }
 
       // ---- its pages, and this pair's share of them: every other one, or
       // one stage without data
       int n_row;
-      if (listed) {
+      const int n_pages = (req.len + kPage - 1) / kPage;
+      if (single) {
         const int32_t* list =
             args.topk_idx + (static_cast<int64_t>(g) * args.total_q + token) * args.topk;
-        const int n_pages = (req.len + kPage - 1) / kPage;
         int32_t v[4];
         bool bad = false;
 #pragma unroll
@@ -499,12 +583,15 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
         }
         if (bad) report(args.status, LS_DEVERR_PAGE_INDEX);
         __syncwarp();
-        n_row = warp_compact_pages(v, ps->pages, lane);
+        n_row = warp_compact_pages(v, reinterpret_cast<int32_t*>(ps->pages), lane);
         __syncwarp();
+      } else if (listed) {
+        n_row = union_pages(args, ps->pages, token, tokens, g, n_pages, limit, lane);
       } else {
         n_row = limit >= 0 ? limit / kPage + 1 : 0;
       }
-      const int lo = min(at.unit, n_row) + pair, hi = min(unit_end, n_row);
+      // (more pages than units: max_seqlen_k was no bound; the last unit takes them)
+      const int lo = min(at.unit, n_row) + pair, hi = unit_end < units ? min(unit_end, n_row) : n_row;
       const int count = max(0, (hi - lo + 1) >> 1);
       const int n_stages = max(1, count);
 
@@ -514,10 +601,14 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
         PageDesc d;
         d.y = -1;
         d.key0 = 0;
+        d.tokens = tokens;
+        d.mask = (1u << tokens) - 1;
         float ks = 1.f, vs = 1.f;
         if (base + lane < count) {
           const int i = lo + 2 * (base + lane);
-          const int logical = listed ? ps->pages[i] : i;
+          const uint32_t entry = listed ? ps->pages[i] : i;
+          const int logical = listed && !single ? entry >> 16 : entry;
+          if (listed && !single) d.mask = entry & 0xFFFF;
           const int page = __ldg(table + logical);
           d.key0 = logical * kPage;
           if (page >= 0 && page < args.num_pages) {
@@ -590,14 +681,14 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
         fill += n;
       }
       // ---- on to the next row
-      left -= unit_end - at.unit;
+      left -= unit_end + kPagedRowCost - done;
       at.unit = 0;
-      if (listed) {
+      if (single) {
         if (++at.token == rows_listed) {
           at.token = 0;
           ++at.group;
         }
-      } else if (++at.token >= req.nq) {
+      } else if ((at.token += pack) >= req.nq) {
         at.token = 0;
         if (++at.group == G) {
           at.group = 0;
@@ -658,12 +749,15 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
   int slot = 0, stage = 0, row_parity = 0;
   uint32_t phase = 0;
   // The first row is known from the start: its queries load while its pages do.
-  int token = sm->start.token, group = sm->start.group;
-  if (!listed) token += __ldg(args.cu_q + sm->start.b);
+  int token = sm->start.token, group = sm->start.group, tokens = 1;
+  if (!single) {
+    const Request r = load_request(args, sm->start.b);
+    tokens = min(pack, r.nq - token);
+    token += r.q0;
+  }
+  const int tok0 = gq / Hg, tok1 = (gq + 8) / Hg;  // tokens of this lane's tile rows
   while (true) {
-    load_query<kHalf>(
-        args.q + (static_cast<int64_t>(token) * args.num_heads + group * Hg) * 128 + 32 * c, gq, Hg,
-        args.scale_log2, qa, &f0, &f1);
+    load_query<kHalf>(args, token, group, kShared ? tokens : 1, gq, c, qa, &f0, &f1);
 #pragma unroll
     for (int j = 0; j < 16; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
     float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
@@ -672,8 +766,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
       if (!mbar_sleep(&ps->full[slot], phase, args.status, abort_flag)) return;
       const PageDesc& desc = ps->desc[stage++ % kDescs];
       flags = desc.row;
+      if (flags & kStop) return;  // a range that holds no row
 
-      // Keys of this warp that the row may see: all 32, some or none.
+      // Keys of this warp that the last token may see: all 32, some or none.
       const int seen = desc.limit - (desc.key0 + key_base) + 1;
       if ((flags & kData) && seen > 0) {
         const uint32_t st = smem_u32(ring + slot * kStageBytes);
@@ -692,14 +787,22 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
         // The values of the first 16 keys are converted while the products run.
         uint32_t vb[16][2];
         load_values(st, v_off0, v_off1, 0, c, seen, vb);
-        // ---- keys past the limit
-        const bool ragged = seen < 32;
-        if (ragged) {
+        // ---- keys past a token's limit, and tokens that do not list the page
+        // (kShared; the first token sees `back` keys less than the last)
+        const int back = kShared && args.causal ? tokens - 1 : 0;
+        const uint32_t mask = kShared ? desc.mask : 1;
+        const bool partial = seen - back < 32 || (kShared && mask != (1u << tokens) - 1);
+        if (partial) {
+          int seen0 = seen, seen1 = seen;
+          if (kShared) {
+            seen0 = (mask >> tok0 & 1) ? seen - max(back - tok0, 0) : 0;
+            seen1 = (mask >> tok1 & 1) ? seen - max(back - tok1, 0) : 0;
+          }
 #pragma unroll
           for (int n = 0; n < 4; ++n)
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-              if (n * 8 + 2 * c + (e & 1) >= seen) sc[n][e] = -INFINITY;
+              if (n * 8 + 2 * c + (e & 1) >= (e < 2 ? seen0 : seen1)) sc[n][e] = -INFINITY;
         }
         // ---- online softmax in the log2 domain
         const float k0 = f0 * desc.k_scale, k1 = f1 * desc.k_scale, v_log2 = desc.v_log2;
@@ -759,9 +862,39 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
         l0 = fmaf(sum0, desc.v_inv, l0);
         if (!kHalf) l1 = fmaf(sum1, desc.v_inv, l1);
         // ---- O += P V, the other 16 keys converted behind the first product
-        mma_values(o, pa[0], vb);
-        load_values(st, v_off0, v_off1, 1, c, seen, vb);
-        mma_values(o, pa[1], vb);
+        if (kShared && partial && tokens > 1 &&
+            has_nan(st + kTileBytes + key_base * 128, min(seen, 32), lane)) {
+          // A value that some token does not see is NaN, and 0 * NaN would
+          // reach its rows: one token at a time, without the others' keys.
+          for (int t = 0; t < tokens; ++t) {
+            if (!(mask >> t & 1)) continue;
+            const int seen_t = seen - max(back - t, 0);
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              uint32_t p[4];
+#pragma unroll
+              for (int i = 0; i < 4; ++i) p[i] = ((i & 1) ? tok1 : tok0) == t ? pa[u][i] : 0;
+              load_values(st, v_off0, v_off1, u, c, seen_t, vb);
+#pragma unroll
+              for (int j = 0; j < 16; ++j) {
+                float d[4] = {0.f, 0.f, 0.f, 0.f};
+                mma_f16_16816(d, p, vb[j][0], vb[j][1]);
+                if (tok0 == t) {
+                  o[j][0] += d[0];
+                  o[j][1] += d[1];
+                }
+                if (tok1 == t) {
+                  o[j][2] += d[2];
+                  o[j][3] += d[3];
+                }
+              }
+            }
+          }
+        } else {
+          mma_values(o, pa[0], vb);
+          load_values(st, v_off0, v_off1, 1, c, seen, vb);
+          mma_values(o, pa[1], vb);
+        }
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&ps->empty[slot]);
@@ -817,7 +950,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
 #pragma unroll
       for (int w = 0; w < kWarps; ++w)
         lt += m_part[w][row] == -INFINITY ? 0.f : l_part[w][row] * ex2(m_part[w][row] - mt);
-      if (row < Hg) {
+      if (row < (kShared ? Hg * tokens : Hg)) {
         float4 sum[4];
         const int rswz = (seg >> 1) | ((row & 1) << 2);
 #pragma unroll
@@ -839,7 +972,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
           if (seg == 0)
             *reinterpret_cast<float2*>(args.part_ml + prow * 2) = make_float2(mt, lt);
         } else {
-          const int h = group * Hg + row;
+          const int h = group * Hg + (kShared ? row % Hg : row);
+          const int t = token + (kShared ? row / Hg : 0);
           const float f = mt == -INFINITY ? 0.f : 1.f / lt;
           uint4 packed[2];
           uint32_t* pw = reinterpret_cast<uint32_t*>(packed);
@@ -849,11 +983,11 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
             pw[2 * k + 1] = pack_bf16x2(sum[k].z * f, sum[k].w * f);
           }
           uint4* dst = reinterpret_cast<uint4*>(
-              args.out + (static_cast<int64_t>(token) * args.num_heads + h) * 128 + 16 * seg);
+              args.out + (static_cast<int64_t>(t) * args.num_heads + h) * 128 + 16 * seg);
           dst[0] = packed[0];
           dst[1] = packed[1];
           if (args.lse != nullptr && seg == 0)
-            args.lse[static_cast<int64_t>(h) * args.total_q + token] =
+            args.lse[static_cast<int64_t>(h) * args.total_q + t] =
                 mt == -INFINITY ? INFINITY : (mt + log2f(lt)) * 0.69314718055994531f;
         }
       }
@@ -864,6 +998,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
     const PageDesc& next = ps->desc[stage % kDescs];
     if (next.row & kStop) return;
     token = next.token;
+    if (kShared) tokens = next.tokens;
     group = (next.row >> 4) & 0xFFFF;
   }
 }
@@ -881,12 +1016,14 @@ __device__ __forceinline__ float4 load_part(const float* p) {
   return x;
 }
 
-// Writes one joined row of one head: lane l holds its dims 4l .. 4l + 3.
+// Writes one joined tile row (head `head` % heads of the tile's token `head` /
+// heads): lane l holds its dims 4l .. 4l + 3.
 __device__ __forceinline__ void write_row(const PagedAttnArgs& args, int row, int head, int lane,
                                           float4 o, float m, float l) {
   const float f = m == -INFINITY ? 0.f : 1.f / l;
-  const int64_t token = row / args.num_groups;
-  const int h = (row % args.num_groups) * args.heads_per_group + head;
+  const int heads = args.heads_per_group;
+  const int64_t token = row / args.num_groups + head / heads;
+  const int h = (row % args.num_groups) * heads + head % heads;
   uint2 packed;
   packed.x = pack_bf16x2(o.x * f, o.y * f);
   packed.y = pack_bf16x2(o.z * f, o.w * f);
@@ -916,7 +1053,7 @@ __global__ void __launch_bounds__(32 * kMergeWarps) paged_merge_many_kernel(
   __shared__ float4 sum[kMergeWarps][32];
   __shared__ float weight[kPagedMaxRanges];
   __shared__ float warp_m[kMergeWarps], warp_l[kMergeWarps];
-  __shared__ int first, behind;
+  __shared__ int first, behind, tokens;
   static_assert(kPagedMaxRanges <= 32 * kMergeWarps, "one thread per range");
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int row = blockIdx.x, h = blockIdx.y;
@@ -932,11 +1069,14 @@ __global__ void __launch_bounds__(32 * kMergeWarps) paged_merge_many_kernel(
     ml = mls[static_cast<int64_t>(2 * tid) * 16 + h];
     begin = mls[static_cast<int64_t>(2 * tid + 1) * 16 + h];
   }
-  if (head.x == row) first = tid;
+  if (head.x == row) {
+    first = tid;
+    tokens = head.y >> 1;
+  }
   __syncthreads();
   const int j = first;
-  if (j >= ranges) return;  // the row is whole in one range
-  if (tid > j && tid < ranges && head.y != 0) atomicMin(&behind, tid);
+  if (j >= ranges || h >= args.heads_per_group * tokens) return;  // the row is whole in one range
+  if (tid > j && tid < ranges && (head.y & 1)) atomicMin(&behind, tid);
   __syncthreads();
   const int n = min(behind, ranges - 1) - j + 1;
   if (tid == j) ml = begin;
@@ -994,9 +1134,9 @@ __global__ void __launch_bounds__(256) paged_merge_few_kernel(
   const int h = blockIdx.y * 8 + (threadIdx.x >> 5);
   allow_next_launch();
   wait_for_inputs();
-  if (h >= args.heads_per_group) return;
-  const int row = args.headers[j].x;
-  if (row < 0) return;  // most ranges here
+  const int2 head = args.headers[j];
+  const int row = head.x;
+  if (row < 0 || h >= args.heads_per_group * (head.y >> 1)) return;  // most ranges here
   float m = -INFINITY, l = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   bool more = true;
@@ -1005,7 +1145,7 @@ __global__ void __launch_bounds__(256) paged_merge_few_kernel(
     int ends_row = 1;
     float2 ml = make_float2(-INFINITY, 0.f);
     if (k < ranges) {
-      ends_row = args.headers[k].y;
+      ends_row = args.headers[k].y & 1;
       ml = reinterpret_cast<const float2*>(args.part_ml)[part_row(j, base + lane, h)];
     }
     const uint32_t ends = __ballot_sync(0xffffffffu, base + lane > 0 && ends_row != 0);
@@ -1044,7 +1184,7 @@ __global__ void __launch_bounds__(256) paged_merge_few_kernel(
 // Once per device: the register split of the kernel draws on what the block is
 // launched with, so a build that gives it fewer registers must not run; and the
 // shared memory limit.
-template <bool kHalf>
+template <bool kHalf, bool kShared>
 cudaError_t prepare_attn_kernel() {
   static std::atomic<uint64_t> ready[4];  // a bit per device, set once it is done there
   int device = 0;
@@ -1054,25 +1194,26 @@ cudaError_t prepare_attn_kernel() {
   const bool tracked = device >= 0 && device < 256;
   if (tracked && (ready[device >> 6].load(std::memory_order_acquire) & bit)) return cudaSuccess;
   cudaFuncAttributes attr;
-  err = cudaFuncGetAttributes(&attr, paged_attn_kernel<kHalf>);
+  err = cudaFuncGetAttributes(&attr, paged_attn_kernel<kHalf, kShared>);
   if (err != cudaSuccess) return err;
   if (attr.numRegs != kLaunchRegs) return cudaErrorInvalidConfiguration;
-  err = cudaFuncSetAttribute(paged_attn_kernel<kHalf>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+  err = cudaFuncSetAttribute(paged_attn_kernel<kHalf, kShared>,
+                             cudaFuncAttributeMaxDynamicSharedMemorySize,
                              static_cast<int>(paged_smem_bytes()));
   if (err == cudaSuccess && tracked) ready[device >> 6].fetch_or(bit, std::memory_order_release);
   return err;
 }
 
-template <bool kHalf>
+template <bool kHalf, bool kShared>
 cudaError_t launch_attn_kernel(const PagedAttnArgs& args, int ranges, cudaStream_t stream) {
-  cudaError_t err = prepare_attn_kernel<kHalf>();
+  cudaError_t err = prepare_attn_kernel<kHalf, kShared>();
   if (err != cudaSuccess) return err;
   const int ctas = (ranges + kTeams - 1) / kTeams;
-  err = launch_early(paged_attn_kernel<kHalf>, dim3(ctas), dim3(kThreads), paged_smem_bytes(),
+  err = launch_early(paged_attn_kernel<kHalf, kShared>, dim3(ctas), dim3(kThreads), paged_smem_bytes(),
                      stream, args);
   if (err != cudaSuccess) return err;
   const int64_t rows = args.total_q * args.num_groups;
-  const int heads = args.heads_per_group;
+  const int heads = args.heads_per_group * args.pack;  // rows of a tile
   ranges = ctas * kTeams;
   if (rows * 16 < ranges)  // more than 16 parts a row
     return launch_early(paged_merge_many_kernel, dim3(static_cast<unsigned>(rows), heads),
@@ -1082,8 +1223,12 @@ cudaError_t launch_attn_kernel(const PagedAttnArgs& args, int ranges, cudaStream
 }
 
 cudaError_t launch_paged_attn(const PagedAttnArgs& args, int ranges, cudaStream_t stream) {
-  return args.heads_per_group <= 8 ? launch_attn_kernel<true>(args, ranges, stream)
-                                   : launch_attn_kernel<false>(args, ranges, stream);
+  const bool half = args.heads_per_group * args.pack <= 8;
+  if (args.pack > 1)
+    return half ? launch_attn_kernel<true, true>(args, ranges, stream)
+                : launch_attn_kernel<false, true>(args, ranges, stream);
+  return half ? launch_attn_kernel<true, false>(args, ranges, stream)
+              : launch_attn_kernel<false, false>(args, ranges, stream);
 }
 
 }  // namespace ls

@@ -496,6 +496,54 @@ def test_listed_rows_with_padding_and_no_causal_limit():
     run_attend(32, 2, seq, nq, idx=idx, pad=4, causal=False)
 
 
+@pytest.mark.parametrize("H, G", [(4, 1), (16, 2), (6, 2), (3, 1), (16, 16), (32, 2), (9, 1)])
+@pytest.mark.parametrize("listed", [False, True])
+def test_tokens_of_a_request_share_tiles(H, G, listed):
+    """Drafts and chunks: tiles of several tokens, the last of them partly filled,
+    rows before position 0, requests of no and of few tokens."""
+    seq, nq = [300, 0, 64, 7, 1500], [5, 0, 17, 9, 33]
+    idx = None
+    if listed:
+        idx = page_lists(seq, nq, G, 9, 3, "repeats")
+        idx[:, 3] = -1
+    for causal in (True, False):
+        run_attend(H, G, seq, nq, idx=idx, causal=causal, seed=H)
+
+
+def test_long_requests_keep_single_lists():
+    """Lists of requests beyond the shared table (512 pages), several tokens each."""
+    seq, nq = [33000, 200], [3, 4]
+    run_attend(8, 2, seq, nq, idx=page_lists(seq, nq, 2, 40, 3, "ascending"), seed=1)
+
+
+@pytest.mark.parametrize("listed", [False, True])
+def test_nan_stays_with_the_rows_that_see_it(listed):
+    """A NaN value reaches the tokens that attend to it and no others of their tile."""
+    H, G, length, n = 4, 1, 200, 4
+    codes, scales, table = make_cache([length], G, 5, nan_tail=False)
+    raw = [c.view(torch.uint8) for c in codes]
+    last = table[0][length // PAGE]
+    raw[1][last, 0, (length - 2) % PAGE, 7] = 0x7F   # seen by the last two tokens
+    raw[0][last, 0, (length - 1) % PAGE, 9] = 0xFF   # a key that the last token sees
+    idx = None
+    if listed:
+        raw[1][table[0][1], 0, 5, 3] = 0xFF          # in a page that tokens 1 and 3 list
+        idx = torch.tensor([[[0, 3, -1], [0, 1, 3], [0, 2, 3], [1, 3, -1]]], dtype=torch.int32)
+    gen = torch.Generator().manual_seed(3)
+    q = torch.randn(n, H, 128, generator=gen).bfloat16()
+    got = ops.paged_attn(q.to(DEV), codes[0].to(DEV), codes[1].to(DEV), scales[0].to(DEV),
+                         scales[1].to(DEV), i32(table), i32([length]), i32([0, n]), n, length,
+                         topk_idx=None if idx is None else idx.to(DEV)).double().cpu()
+    want, _, bounds = ora.attend(q, codes[0].float(), codes[1].float(), scales[0], scales[1], table,
+                                 [length], [0, n], idx)
+    # NaN in the sum of a dim at any weight, as 0 * NaN; whole rows for the NaN key
+    assert torch.equal(got.isnan(), want.isnan())
+    assert bool(want.isnan()[n - 1].all()) and not bool(want.isnan()[0].any())
+    ok = ~want.isnan()
+    err = (got - want).abs()
+    assert bool((err[ok] <= tolerance(want, bounds, length)[ok]).all())
+
+
 def test_bad_pages_are_passed_over_and_reported():
     codes, scales, table = make_cache([300, 64], 2, 3)
     table[0][1] = 10 ** 6
