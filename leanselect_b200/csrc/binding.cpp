@@ -97,7 +97,7 @@ PyObject* plan_pages(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
       !plain(table, at::kInt, dev) || table->dim() != 2 || table->size(0) != batch ||
       table->size(1) < 1 || !fits32(table->size(1)) || !plain(pool, at::kInt, dev) ||
       pool->dim() != 1 || !fits32(pool->size(0)) || !plain(head, at::kInt, dev) ||
-      head->numel() != 1 || !vec(status, at::kInt, dev, 1) || total < 0)
+      head->numel() != 1 || !vec(status, at::kInt, dev, 1) || !fits32(total))
     Py_RETURN_NONE;
   at::AutoDispatchBelowADInplaceOrView below;
   const c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(dev));

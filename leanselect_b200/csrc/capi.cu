@@ -835,7 +835,8 @@ int ls_paged_attn(const uint16_t* q, const uint8_t* k_pages, const uint8_t* v_pa
                   float* lse, int32_t* status, void* stream) {
   const int rc = check_cache(k_pages, v_pages, k_scale, v_scale, num_pages, num_kv_heads, head_dim);
   if (rc != LS_OK) return rc;
-  LS_REQUIRE(q && block_table && seq_lens && cu_seqlens_q && out, "null argument");
+  LS_REQUIRE(block_table && seq_lens && cu_seqlens_q, "null argument");
+  LS_REQUIRE(total_q == 0 || (q && out), "null q or out");
   LS_REQUIRE(batch >= 1 && max_blocks >= 1 && total_q >= 0, "bad sizes");
   LS_REQUIRE(max_blocks <= (1 << 24), "max_blocks out of range");
   LS_REQUIRE(max_seqlen_q >= 0 && max_seqlen_k >= 0, "bad max_seqlen");

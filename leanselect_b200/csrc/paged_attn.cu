@@ -61,9 +61,7 @@ struct __align__(16) PageDesc {
   int limit;       // last position the tile's last token sees
   int token;       // the tile's first token
   int row;         // StageFlag | group << 4 | (workspace part + 1) << 20, part -1: none
-  int y;           // the page's first row in the tensor maps (-1: no data)
-  int tokens;      // tokens of the tile
-  uint32_t mask;   // those of them that list the page
+  uint32_t tile;   // tokens of the tile << 16 | those of them that list the page
 };
 constexpr int kDescs = 64;  // a batch of 32 never reaches the stages still in the ring
 
@@ -78,6 +76,7 @@ struct PairSmem {
   uint64_t full[kStages];
   uint64_t empty[kStages];
   PageDesc desc[kDescs];
+  int y[kDescs];  // the pages' first rows in the tensor maps (-1: no data)
   // listed: the row's sorted pages; for tiles of several tokens page << 16 |
   // the tokens that list it
   uint32_t pages[kPagedMaxUnion];
@@ -599,20 +598,19 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
       for (int base = 0; base < n_stages && ok; base += 32) {
         // 32 pages at once, one per lane: table entry, then both scales.
         PageDesc d;
-        d.y = -1;
+        int y = -1;
         d.key0 = 0;
-        d.tokens = tokens;
-        d.mask = (1u << tokens) - 1;
+        uint32_t mask = (1u << tokens) - 1;
         float ks = 1.f, vs = 1.f;
         if (base + lane < count) {
           const int i = lo + 2 * (base + lane);
           const uint32_t entry = listed ? ps->pages[i] : i;
           const int logical = listed && !single ? entry >> 16 : entry;
-          if (listed && !single) d.mask = entry & 0xFFFF;
+          if (listed && !single) mask = entry & 0xFFFF;
           const int page = __ldg(table + logical);
           d.key0 = logical * kPage;
           if (page >= 0 && page < args.num_pages) {
-            d.y = (page * G + g) * kPage;
+            y = (page * G + g) * kPage;
             ks = __ldg(args.k_scale + static_cast<int64_t>(page) * G + g);
             vs = __ldg(args.v_scale + static_cast<int64_t>(page) * G + g);
           } else {
@@ -624,7 +622,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
         const int early = min(n, kStages);
         int y0[kStages];
 #pragma unroll
-        for (int j = 0; j < kStages; ++j) y0[j] = __shfl_sync(0xffffffffu, d.y, j);
+        for (int j = 0; j < kStages; ++j) y0[j] = __shfl_sync(0xffffffffu, y, j);
         int s0 = slot;
         uint32_t p0 = phase;
         if (lane == 0) {
@@ -652,8 +650,12 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
         d.token = token;
         const int nth = base + lane;
         d.row = (nth == 0 ? kFirst : 0) | (nth + 1 == n_stages ? kLast : 0) |
-                (d.y >= 0 ? kData : 0) | g << 4 | (part + 1) << 20;
-        if (lane < n) ps->desc[(fill + lane) % kDescs] = d;
+                (y >= 0 ? kData : 0) | g << 4 | (part + 1) << 20;
+        d.tile = static_cast<uint32_t>(tokens) << 16 | mask;
+        if (lane < n) {
+          ps->desc[(fill + lane) % kDescs] = d;
+          ps->y[(fill + lane) % kDescs] = y;
+        }
         __syncwarp();
         if (lane == 0) {
           for (int j = 0; j < n; ++j) {
@@ -663,7 +665,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
             } else {
               ok = ok && mbar_sleep(&ps->empty[slot], phase, args.status, abort_flag);
               if (!ok) break;
-              const int y = ps->desc[(fill + j) % kDescs].y;
+              const int y = ps->y[(fill + j) % kDescs];
               if (y >= 0) {
                 mbar_arrive_expect_tx(&ps->full[slot], kStageBytes);
                 load_page(args, ring + slot * kStageBytes, &ps->full[slot], y);
@@ -790,7 +792,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
         // ---- keys past a token's limit, and tokens that do not list the page
         // (kShared; the first token sees `back` keys less than the last)
         const int back = kShared && args.causal ? tokens - 1 : 0;
-        const uint32_t mask = kShared ? desc.mask : 1;
+        const uint32_t mask = kShared ? desc.tile & 0xFFFF : 1;
         const bool partial = seen - back < 32 || (kShared && mask != (1u << tokens) - 1);
         if (partial) {
           int seen0 = seen, seen1 = seen;
@@ -998,7 +1000,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
     const PageDesc& next = ps->desc[stage % kDescs];
     if (next.row & kStop) return;
     token = next.token;
-    if (kShared) tokens = next.tokens;
+    if (kShared) tokens = next.tile >> 16;
     group = (next.row >> 4) & 0xFFFF;
   }
 }

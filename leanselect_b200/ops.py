@@ -620,8 +620,8 @@ def plan_pages(context_lens: torch.Tensor, new_lens: torch.Tensor, block_table: 
     if free.ndim != 1 or head.numel() != 1:
         raise ValueError("free_pages must be a vector and free_head one number")
     total_new = int(total_new)
-    if total_new < 0:
-        raise ValueError("total_new must not be negative")
+    if not 0 <= total_new < 1 << 31:
+        raise ValueError("total_new must lie in [0, 2^31)")
     # The five int32 results share one allocation.
     ints = torch.empty(3 * batch + 3, dtype=torch.int32, device=dev)
     seq, cu_q, cu_blocks, head_out = ints.split([batch, batch + 1, batch + 1, 1])

@@ -165,6 +165,7 @@ def test_plan_refusals():
                 free_pages=i32([0]), free_head=i32([0]), total_new=1)
     for change in (dict(new_lens=i32([1, 1])), dict(block_table=i32([[-1], [-1]])),
                    dict(block_table=i32([[-1]]).long()), dict(total_new=-1),
+                   dict(total_new=1 << 31),
                    dict(free_head=i32([0, 0])),
                    dict(block_table=i32([[-1] * 4])[:, ::2])):
         with pytest.raises(ValueError):
@@ -414,6 +415,35 @@ def test_dense_ragged_batch(causal):
 def test_rows_without_keys_are_zero():
     """Empty requests, and rows that stand before position 0."""
     run_attend(16, 2, [0, 5, 0, 3], [1, 1, 2, 6])
+
+
+@pytest.mark.parametrize("H, G", [(8, 8), (32, 2)])
+def test_short_rows_between_long_ones(H, G):
+    """Ranges that begin in a row's leading units, hold many short rows or none."""
+    run_attend(H, G, [9000, 1, 1, 5000, 0, 2, 64, 1, 1], [1, 1, 2, 1, 1, 1, 0, 1, 1], seed=3)
+    run_attend(H, G, [1] * 700, [1] * 700, seed=4)
+
+
+@pytest.mark.parametrize("batch", [33, 500])
+@pytest.mark.parametrize("listed", [False, True])
+def test_drafts_of_many_requests(batch, listed):
+    """Batches that the whole block adds up, several tokens each, some none."""
+    gen = torch.Generator().manual_seed(batch)
+    seq = torch.randint(0, 200, (batch,), generator=gen).tolist()
+    nq = torch.randint(0, 4, (batch,), generator=gen).tolist()
+    idx = page_lists(seq, nq, 2, 3, 3, "future") if listed else None
+    run_attend(8, 2, seq, nq, idx=idx, seed=batch)
+
+
+def test_no_rows_and_no_tokens():
+    codes, scales, table = make_cache([64], 2, 3)
+    cache = [codes[0].to(DEV), codes[1].to(DEV), scales[0].to(DEV), scales[1].to(DEV)]
+    q = torch.empty(0, 32, 128, dtype=torch.bfloat16, device=DEV)
+    out, lse = ops.paged_attn(q, *cache, i32(table), i32([64]), i32([0, 0]), 0, 64, return_lse=True)
+    assert out.shape == (0, 32, 128) and lse.shape == (32, 0)
+    plan = ops.plan_pages(i32([64]), i32([0]), i32([[0, -1]]), i32([1]), i32([0]), 0)
+    ops.append_kv(q[:, :2], q[:, :2], plan, *cache)
+    assert plan.slots.numel() == 0 and plan.seq_lens.tolist() == [64]
 
 
 def test_rows_behind_the_last_request_are_left():
