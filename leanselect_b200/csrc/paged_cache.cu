@@ -58,8 +58,12 @@ __device__ __forceinline__ PlanRow plan_row(const PlanArgs& a, int b) {
 // request by binary search.  The thread of a new block's first token writes
 // its block-table entry; a token in the half-filled old block reads that
 // block's entry, which nobody writes.  Integer sums only: the result does not
-// depend on the launch shape.
-template <int kTokens>
+// depend on the launch shape.  Latency bound, a chain of round trips (lengths,
+// page, stores): 2.6 us of device time for 8 decode tokens, 4.1 for 1024, 8.3
+// for the 727K tokens of 64 prompts (11.6 MB of results, 1.8 us at the copy
+// rate; up to four CTAs per SM, as two took 9.1 and ten 10.8, since each repeats
+// the sums; four neighbouring tokens a thread with 16-byte stores took 8.9, and
+// 3.9 instead of 2.6 for small steps).
 __global__ void __launch_bounds__(kPlanThreads) plan_pages_kernel(const __grid_constant__ PlanArgs a) {
   extern __shared__ int32_t plan_smem[];
   int32_t* cu_q = plan_smem;                  // [batch + 1]
@@ -162,66 +166,39 @@ __global__ void __launch_bounds__(kPlanThreads) plan_pages_kernel(const __grid_c
   if (lead && bad) report(a.status, LS_DEVERR_SEQLENS);
   __syncthreads();
 
-  // The page of block `block` of request b, and its table entry when the block
-  // begins in this step (`begins`: the caller holds its first token).
-  const auto page_of = [&](int b, int ctx, int block, bool begins) {
-    if (block >= a.max_blocks) return -1;
-    int32_t* entry = a.block_table + static_cast<int64_t>(b) * a.max_blocks + block;
-    const int had = (ctx + kPage - 1) / kPage;
-    if (block < had) return *entry;
-    const int64_t at = head + cu_need[b] + (block - had);
-    const int32_t page = at < a.num_free ? __ldg(a.free_pages + at) : -1;
-    if (begins) *entry = page;
-    return page;
-  };
-  // kTokens neighbouring tokens a thread: one search and mostly one page for
-  // four, and 16-byte stores (single ones where the arrays are not aligned).
   const int total_new = static_cast<int>(a.total_new);
   const int tokens = static_cast<int>(min(tok_all, a.total_new));
-  const bool wide =
-      kTokens == 4 &&
-      ((reinterpret_cast<uintptr_t>(a.slots) | reinterpret_cast<uintptr_t>(a.positions)) & 15) == 0;
-  const uint32_t stride = gridDim.x * kPlanThreads * kTokens;
-  for (uint32_t at = (blockIdx.x * kPlanThreads + tid) * kTokens;
-       at < static_cast<uint32_t>(total_new); at += stride) {
-    const int i0 = static_cast<int>(at);
-    // Last request whose first token is at or before i0 (empty requests share
-    // their successor's offset and are passed over).
-    int b = 0, top = i0 < tokens ? a.batch - 1 : 0;
-    while (b < top) {
-      const int mid = (b + top + 1) >> 1;
-      if (cu_q[mid] <= i0) b = mid; else top = mid - 1;
-    }
-    int ctx = min(max(__ldg(a.context_lens + b), 0), 1 << 30);
-    int pos = ctx + (i0 - cu_q[b]);
-    if (wide && i0 + 4 <= min(tokens, cu_q[b + 1]) && pos % kPage <= kPage - 4) {
-      const int page = page_of(b, ctx, pos / kPage, pos % kPage == 0);
-      const int64_t s0 = static_cast<int64_t>(page) * kPage + pos % kPage;
-      longlong2* s = reinterpret_cast<longlong2*>(a.slots + i0);
-      longlong2* p = reinterpret_cast<longlong2*>(a.positions + i0);
-      s[0] = page >= 0 ? make_longlong2(s0, s0 + 1) : make_longlong2(-1, -1);
-      s[1] = page >= 0 ? make_longlong2(s0 + 2, s0 + 3) : make_longlong2(-1, -1);
-      p[0] = make_longlong2(pos, pos + 1LL);
-      p[1] = make_longlong2(pos + 2LL, pos + 3LL);
-      continue;
-    }
-#pragma unroll 1
-    for (int i = i0; i < min(i0 + kTokens, total_new); ++i) {
-      int64_t slot = -1;
-      if (i < tokens) {
-        while (i >= cu_q[b + 1]) ++b;
-        if (kTokens > 1) {
-          ctx = min(max(__ldg(a.context_lens + b), 0), 1 << 30);
-          pos = ctx + (i - cu_q[b]);
-        }
-        const int page = page_of(b, ctx, pos / kPage, pos % kPage == 0);
-        if (page >= 0) slot = static_cast<int64_t>(page) * kPage + pos % kPage;
-      } else {
-        pos = 0;
+  for (uint32_t at = blockIdx.x * kPlanThreads + tid; at < static_cast<uint32_t>(total_new);
+       at += gridDim.x * kPlanThreads) {
+    const int i = static_cast<int>(at);
+    int64_t slot = -1;
+    int pos = 0;
+    if (i < tokens) {
+      // Last request whose first token is at or before i (empty requests share
+      // their successor's offset and are passed over).
+      int b = 0, top = a.batch - 1;
+      while (b < top) {
+        const int mid = (b + top + 1) >> 1;
+        if (cu_q[mid] <= i) b = mid; else top = mid - 1;
       }
-      a.slots[i] = slot;
-      a.positions[i] = pos;
+      const int ctx = min(max(__ldg(a.context_lens + b), 0), 1 << 30);
+      pos = ctx + (i - cu_q[b]);
+      const int block = pos / kPage, had = (ctx + kPage - 1) / kPage;
+      if (block < a.max_blocks) {
+        int32_t* entry = a.block_table + static_cast<int64_t>(b) * a.max_blocks + block;
+        int32_t page;
+        if (block < had) {
+          page = *entry;
+        } else {
+          const int64_t from = head + cu_need[b] + (block - had);
+          page = from < a.num_free ? __ldg(a.free_pages + from) : -1;
+          if (pos % kPage == 0) *entry = page;
+        }
+        if (page >= 0) slot = static_cast<int64_t>(page) * kPage + pos % kPage;
+      }
     }
+    a.slots[i] = slot;
+    a.positions[i] = pos;
   }
 }
 
@@ -334,7 +311,11 @@ __device__ __forceinline__ BlockRows find_block(const AppendArgs& a, int64_t ite
 // rescaled by the ratio (exact but for e4m3 subnormals, since scales are powers
 // of two); rows behind r1 are left as they were.  16 threads of 8 values per
 // row; kThreads (per half) is 128 for pages that fill up and 32 for steps of a
-// token or two, where the rest of a larger block would only wait.
+// token or two, where the rest of a larger block would only wait.  Bound by HBM
+// when pages fill up: a prompt of 131072 tokens, 134 MB read and 67 MB written,
+// takes 35 us, 5.8 TB/s, 0.88 of the measured copy rate.  A step of one token a
+// request is a chain of round trips (lengths, slot, scale): 2.2 us of device
+// time for 8 requests, 2.8 for 512 (10.9 with a binary search for the request).
 template <int kThreads>
 __global__ void __launch_bounds__(2 * kThreads, kThreads == 128 ? 3 : 16) append_kv_kernel(const __grid_constant__ AppendArgs a) {
   constexpr int kWarps = kThreads / 32, kRows = kThreads / 16, kPasses = kPage / kRows;
@@ -432,24 +413,17 @@ __global__ void __launch_bounds__(2 * kThreads, kThreads == 128 ? 3 : 16) append
 
 }  // namespace
 
-template <int kTokens>
-cudaError_t launch_plan(const PlanArgs& args, cudaStream_t stream) {
+cudaError_t launch_plan_pages(const PlanArgs& args, cudaStream_t stream) {
   const size_t smem = 2 * sizeof(int32_t) * (static_cast<size_t>(args.batch) + 1);
   if (smem > 40 * 1024) {
     const cudaError_t err =
-        cudaFuncSetAttribute(plan_pages_kernel<kTokens>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+        cudaFuncSetAttribute(plan_pages_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                              static_cast<int>(smem));
     if (err != cudaSuccess) return err;
   }
-  const int64_t per = kTokens * kPlanThreads, want = (args.total_new + per - 1) / per;
+  const int64_t want = (args.total_new + kPlanThreads - 1) / kPlanThreads;
   const unsigned grid = static_cast<unsigned>(want < 1 ? 1 : want > 148 * 4 ? 148 * 4 : want);
-  return launch_early(plan_pages_kernel<kTokens>, dim3(grid), dim3(kPlanThreads), smem, stream, args);
-}
-
-cudaError_t launch_plan_pages(const PlanArgs& args, cudaStream_t stream) {
-  // Four tokens a thread once that still gives every SM a block.
-  return args.total_new >= 148 * 4 * kPlanThreads ? launch_plan<4>(args, stream)
-                                                  : launch_plan<1>(args, stream);
+  return launch_early(plan_pages_kernel, dim3(grid), dim3(kPlanThreads), smem, stream, args);
 }
 
 cudaError_t launch_append_kv(const AppendArgs& args, cudaStream_t stream) {
@@ -458,7 +432,8 @@ cudaError_t launch_append_kv(const AppendArgs& args, cudaStream_t stream) {
   const int64_t blocks = args.total_new < ragged ? args.total_new : ragged;
   if (blocks == 0) return cudaSuccess;
   const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(args.num_groups));
-  // Up to two tokens a request on average: single warps.
+  // Up to two tokens a request on average: single warps (512 tokens of 512
+  // requests 2.8 us against 7.4; a prompt of 131072 tokens 57 us against 35).
   return args.total_new <= 2 * static_cast<int64_t>(args.batch)
              ? launch_early(append_kv_kernel<32>, grid, dim3(64), 0, stream, args)
              : launch_early(append_kv_kernel<128>, grid, dim3(256), 0, stream, args);
