@@ -5,24 +5,49 @@
 // over the keys of the row's pages at positions <= p, with k = ks * code and
 // v = vs * code (e4m3 codes, one ks and vs per (page, group)).
 //
-// A (token, group) row reads 16 KB of codes per page for 16 heads: the path
-// is bound by moving pages, from HBM when caches are long and from L2 when
-// rows share pages.  So the codes go straight from the TMA ring into f16
-// fragments (e4m3 converts exactly), and all scales are folded in elsewhere:
+// A tile of 16 query rows (the heads of one group; with fewer than 16 heads
+// those of several tokens of a request) reads 16 KB of codes per page and
+// does 0.5 MFLOP with them: on long caches HBM bounds it, on lists of pages
+// that rows share the tensor pipe.  So the codes go straight from the TMA
+// ring into f16 fragments (e4m3 converts exactly; the 8-bit form of mma.sync
+// took 1.35 times as long here), and all scales are folded in elsewhere:
 //   * ks multiplies the scores' factor, per page;
 //   * vs is folded into the exponent: P' = 2^(x + log2 vs - M), so that
 //     sum P' code needs no page factor, and the row sum takes P' / vs;
 //   * q is scaled per row by a power of two into f16's range.
 // M is a lazily raised reference (it moves only when x + log2 vs exceeds it
 // by 14 binades; it is set 6 below the maximum), so P' <= 2^14 holds f16's 11
-// bits down to 2^-20 of the largest.  Sums and accumulators are fp32.
+// bits down to 2^-20 of the largest: rounding the weights to f16 costs half a
+// step of 2^-11, less than the bf16 output.  Sums and accumulators are fp32.
 //
-// Work split.  All rows' page lists are laid end to end and cut into equal
-// ranges, one per CTA, two CTAs per SM: ragged batches stay balanced and one
-// long row fills the GPU.  A row inside one range is written at once; the
-// parts of a row cut by range borders go to a workspace and
-// paged_merge_kernel joins them.  The cut depends on the shapes and lengths
-// alone, and no sum uses atomics, so equal calls give equal bits.
+// Work split.  All tiles' pages are laid end to end and cut into equal ranges,
+// two per SM: ragged batches stay balanced and one long row fills the GPU.  A
+// tile inside one range is written at once; the parts of a tile cut by range
+// borders go to a workspace and a second kernel joins them.  The cut depends
+// on the shapes and lengths alone, and no sum uses atomics, so equal calls
+// give equal bits.
+//
+// One CTA per SM holds two teams of four consumer warps with 216 registers a
+// thread (each has a range of its own) and four producer warps with 72: the
+// accumulators of a 16 x 128 tile, the queries and a page's fragments fit
+// without spills, which a fifth warp per CTA at two CTAs per SM (168
+// registers) does not allow.  Two warps of a team share a page, 32 keys each,
+// and the pairs take alternate pages from rings of their own: 64 KB in flight
+// per team, and half the waits and votes per key of 16-key shares.
+//
+// Measured (CUDA-graph replays): 64 ragged requests up to 32768 tokens, 2 x 8
+// heads, 596 MB of codes: 101 us, 5.9 TB/s, 0.90 of the measured copy rate
+// (95 us with all arithmetic taken out).  One request of 131072 tokens, 2 x 16
+// heads, 67 MB: 23.6 us, of which the stream takes 9, launch and first page
+// 4.5, the rows' end 1.2 and the merge 5.  A chunk of 512 tokens with 67 listed
+// pages each, 2 x 16 heads, 16 MB cached: 174 us, 207 TFLOP/s, against 71 us
+// for the page copies alone and 64 us for the products at mma.sync's rate (8
+// cycles per m16n8k16 and SM quarter): two warps per quarter, each a chain of
+// ~2300 cycles a page (wait 280, scores 620, softmax 540, values 500, the rest
+// bookkeeping), keep the tensor pipe 40 % busy.  Tried and dropped there: three teams
+// at 152 registers (152 us, but 5 us more for one long request), the next
+// page's scores formed beside this page's product with V (168-186 us), 16-key
+// shares (226 us).
 #include <atomic>
 
 #include <cuda_fp16.h>
@@ -52,7 +77,7 @@ constexpr int kSumBytes = kWarps * 16 * 128 * 4;  // a team's row sums, one set 
 constexpr float kSlack = 14.f, kHeadroom = 6.f;  // binades, see above
 constexpr float kMinScale = 0x1p-40f, kMaxScale = 0x1p48f;
 
-enum StageFlag { kFirst = 1, kLast = 2, kData = 4, kStop = 8 };
+enum StageFlag { kLast = 1, kData = 2, kStop = 4 };  // a row's last stage; a page in it; no more rows
 
 // What a pair's consumers need to know of one stage.
 struct __align__(16) PageDesc {
@@ -649,8 +674,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
         d.limit = limit;
         d.token = token;
         const int nth = base + lane;
-        d.row = (nth == 0 ? kFirst : 0) | (nth + 1 == n_stages ? kLast : 0) |
-                (y >= 0 ? kData : 0) | g << 4 | (part + 1) << 20;
+        d.row = (nth + 1 == n_stages ? kLast : 0) | (y >= 0 ? kData : 0) | g << 4 | (part + 1) << 20;
         d.tile = static_cast<uint32_t>(tokens) << 16 | mask;
         if (lane < n) {
           ps->desc[(fill + lane) % kDescs] = d;
@@ -1217,7 +1241,10 @@ cudaError_t launch_attn_kernel(const PagedAttnArgs& args, int ranges, cudaStream
   const int64_t rows = args.total_q * args.num_groups;
   const int heads = args.heads_per_group * args.pack;  // rows of a tile
   ranges = ctas * kTeams;
-  if (rows * 16 < ranges)  // more than 16 parts a row
+  // More than 16 parts a row: by row.  2 rows of 131072 keys 23.4 us (by range
+  // 49.8), 8 rows of 65536 34.3 (38.2), 16 rows of 32768 34.1 (34.1), 64 listed
+  // rows 34.4 (24.8).
+  if (rows * 16 < ranges)
     return launch_early(paged_merge_many_kernel, dim3(static_cast<unsigned>(rows), heads),
                         dim3(32 * kMergeWarps), 0, stream, args, ranges);
   return launch_early(paged_merge_few_kernel, dim3(ranges, (heads + 7) / 8), dim3(256), 0, stream,

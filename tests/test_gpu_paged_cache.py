@@ -540,6 +540,18 @@ def test_tokens_of_a_request_share_tiles(H, G, listed):
         run_attend(H, G, seq, nq, idx=idx, causal=causal, seed=H)
 
 
+@pytest.mark.parametrize("kind", ["ascending", "shuffled", "repeats", "future", "empty"])
+@pytest.mark.parametrize("H, G", [(4, 1), (16, 2), (6, 2), (3, 1)])
+def test_lists_that_overlap_are_joined(kind, H, G):
+    """Lists three times as long as the requests' pages, for many rows: one tile holds
+    several tokens and walks the union of their pages."""
+    seq, nq = [1500, 64, 0, 700, 7], [40, 17, 0, 33, 9]
+    idx = page_lists(seq, nq, G, 128, 4, kind)
+    idx = torch.nn.functional.pad(idx, (0, 0, 0, 21), value=0)   # rows behind the last request
+    for causal in (True, False):
+        run_attend(H, G, seq, nq, idx=idx, causal=causal, seed=G, pad=21)
+
+
 def test_long_requests_keep_single_lists():
     """Lists of requests beyond the shared table (512 pages), several tokens each."""
     seq, nq = [33000, 200], [3, 4]
@@ -572,6 +584,44 @@ def test_nan_stays_with_the_rows_that_see_it(listed):
     ok = ~want.isnan()
     err = (got - want).abs()
     assert bool((err[ok] <= tolerance(want, bounds, length)[ok]).all())
+
+
+def test_nan_and_bad_pages_in_joined_lists():
+    """As above for lists that are joined: four tokens with one key set each, and a bad page."""
+    H, G, length, n = 4, 1, 200, 4
+    codes, scales, table = make_cache([length], G, 5, nan_tail=False)
+    raw = [c.view(torch.uint8) for c in codes]
+    raw[1][table[0][3], 0, 198 % PAGE, 7] = 0x7F      # seen by the last two tokens
+    raw[0][table[0][3], 0, 199 % PAGE, 9] = 0xFF      # a key that the last token sees
+    raw[1][table[0][1], 0, 5, 3] = 0xFF               # in a page that tokens 1 and 3 list
+    idx = torch.full((1, 100, 128), -1, dtype=torch.int32)
+    for i, pages in enumerate([[0, 3], [0, 1, 3], [0, 2, 3], [3, 1]]):
+        idx[0, i, 5:5 + len(pages)] = torch.tensor(pages, dtype=torch.int32)
+    gen = torch.Generator().manual_seed(3)
+    q = torch.randn(100, H, 128, generator=gen).bfloat16()
+
+    def both():
+        out = torch.full_like(q, 2.0, device=DEV)
+        ops.paged_attn(q.to(DEV), codes[0].to(DEV), codes[1].to(DEV), scales[0].to(DEV),
+                       scales[1].to(DEV), i32(table), i32([length]), i32([0, n]), n, length,
+                       topk_idx=idx.to(DEV), out=out)
+        assert bool((out[n:] == 2.0).all())
+        want, _, bounds = ora.attend(q[:n], codes[0].float(), codes[1].float(), scales[0],
+                                     scales[1], table, [length], [0, n], idx[:, :n])
+        got = out[:n].double().cpu()
+        assert torch.equal(got.isnan(), want.isnan())
+        ok = ~want.isnan()
+        assert bool(((got - want).abs()[ok] <= tolerance(want, bounds, length)[ok]).all())
+        return want
+
+    want = both()
+    assert bool(want.isnan()[3].all()) and bool(want.isnan()[1, :, 3].all())
+    assert not bool(want.isnan()[0].any())
+    table[0][2] = 10 ** 6
+    idx[0, 2, 0] = 9                                  # past the request's pages
+    both()
+    with pytest.raises(_native.LeanSelectError, match="PAGE_INDEX"):
+        ops.check_status(DEV)
 
 
 def test_bad_pages_are_passed_over_and_reported():
