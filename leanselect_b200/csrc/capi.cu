@@ -902,14 +902,15 @@ int ls_paged_attn(const uint16_t* q, const uint8_t* k_pages, const uint8_t* v_pa
   // joined for that where a table of the request's pages fits on chip, where
   // they must overlap threefold (one visit for several tokens masks per page
   // and costs twice as much: 512 tokens of 2 x 2 heads with 96 of 256 pages
-  // each 156 us against 204, with 96 of 384 pages 220 against 212) and where 32
-  // or more listed pages per range hide the joining (32 tokens of 2 x 4 heads,
-  // 32 of 42 pages: 19 us against 14).
+  // each 156 us against 204, with 96 of 384 pages 220 against 212) and where 30
+  // pages per range, rows' own cost included, hide the joining (512 tokens of 2
+  // x 4 heads over 5 pages 19 us against 27; 128 of 2 x 1 heads with 16 of 16
+  // pages 20 against 18, 32 of 2 x 4 with 32 of 42 pages 19 against 14).
   a.pack = 1;
   if (max_seqlen_q > 1) {
     const int tokens = std::min(16 / hg, static_cast<int>(max_seqlen_q));
-    if (topk == 0 || (most_pages <= kPagedMaxUnion && int64_t{tokens} * topk >= 3 * most_pages &&
-                      total_q * num_kv_heads * topk >= int64_t{32} * 2 * sms))
+    if (topk == 0 || (most_pages <= kPagedMaxUnion && int64_t{tokens} * a.units >= 3 * most_pages &&
+                      total_q * num_kv_heads * (a.units + kPagedRowCost) >= int64_t{30} * 2 * sms))
       a.pack = tokens;
   }
   const int64_t per_row = topk > 0 ? a.units : most_pages;
