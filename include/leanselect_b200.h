@@ -453,7 +453,7 @@ int ls_plan_pages(const int32_t* context_lens, const int32_t* new_lens, int32_t 
  * (ties to even, saturating; NaN stays NaN and does not count for s).  Rows
  * of a page behind the request's last token are left as they were, tokens
  * with slot -1 are not stored.  A page written here must belong to one
- * request only.
+ * block of one request.
  */
 int ls_append_kv(const uint16_t* k, const uint16_t* v, int64_t k_stride, int64_t v_stride,
                  int64_t total_new, int32_t batch, int32_t num_kv_heads, int32_t head_dim,
@@ -475,10 +475,15 @@ int ls_append_kv(const uint16_t* k, const uint16_t* v, int64_t k_stride, int64_t
  * are left as they were.  Scales are read clamped to [2^-40, 2^48].  q and
  * out [total_q, H, 128] bf16, lse [H, total_q] fp32 (nullable); scale <= 0
  * selects 128^-0.5.  Requires 1 <= H/G <= 16, topk <= LS_MAX_TOPK.
- * max_seqlen_q / max_seqlen_k bound nq and seq_lens.  `workspace` (16-byte
- * aligned) holds ls_paged_attn_workspace_bytes() bytes; calls that may overlap
- * need one each.  Block-table entries outside [0, num_pages) and list entries
- * past the request's pages are passed over (LS_DEVERR_PAGE_INDEX).
+ * max_seqlen_q / max_seqlen_k bound nq and seq_lens; the work is scheduled by
+ * them, and with H/G <= 8 and max_seqlen_q > 1 neighbouring tokens of a request
+ * may share their reads.  total_q * G * (max_blocks or topk, + 4) must stay
+ * below 2^31.  `workspace` (16-byte aligned) holds
+ * ls_paged_attn_workspace_bytes() bytes; calls that may overlap need one each.
+ * Block-table entries outside [0, num_pages) and list entries past the
+ * request's pages are passed over (LS_DEVERR_PAGE_INDEX; also raised for pages
+ * past the 512th when lists are shared and max_seqlen_k was no bound).  Equal
+ * calls give equal bits; how a row's sum is split depends on the whole batch.
  */
 size_t ls_paged_attn_workspace_bytes(void);
 int ls_paged_attn(const uint16_t* q, const uint8_t* k_pages, const uint8_t* v_pages,
