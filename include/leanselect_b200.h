@@ -419,7 +419,7 @@ int ls_sparse_attn_gather_only(const uint16_t* q, const uint16_t* k, const uint1
  * ls_plan_pages -- pages, slots and positions of one step.  Request b holds
  * context_lens[b] tokens and adds new_lens[b] (>= 0); its tokens are packed
  * one request after the other.  Writes
- *   seq_lens [batch]         context + new tokens
+ *   seq_lens [batch]         context + new tokens (not an input's buffer)
  *   cu_seqlens_q [batch+1]   prefix sums of new_lens
  *   cu_blocks [batch+1]      prefix sums of the pages each request writes
  *   positions [total_new]    a token's position in its request

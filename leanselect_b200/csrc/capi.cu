@@ -737,6 +737,7 @@ int ls_plan_pages(const int32_t* context_lens, const int32_t* new_lens, int32_t 
   LS_REQUIRE(total_new == 0 || (slots && positions), "null slots or positions");
   if (batch > LS_MAX_PLAN_BATCH)
     return fail(LS_ERR_UNSUPPORTED, "batch exceeds LS_MAX_PLAN_BATCH");
+  LS_REQUIRE(seq_lens != context_lens && seq_lens != new_lens, "seq_lens must not be an input");
   PlanArgs a{};
   a.context_lens = context_lens;
   a.new_lens = new_lens;

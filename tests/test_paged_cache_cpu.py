@@ -36,6 +36,7 @@ PLAN = [FAKE, FAKE, 4, FAKE, 8, FAKE, 16, FAKE, 100, FAKE, FAKE, FAKE, FAKE, FAK
     ({8: 1 << 31}, INVALID, b"total_new"),
     ({12: None}, INVALID, b"slots"),
     ({2: _native.LS_MAX_PLAN_BATCH + 1}, UNSUPPORTED, b"LS_MAX_PLAN_BATCH"),
+    ({}, INVALID, b"seq_lens must not be an input"),
 ])
 def test_plan_refusals(changes, code, text):
     refused("ls_plan_pages", PLAN, changes, code, text)
