@@ -380,6 +380,10 @@ __device__ __forceinline__ Request load_request(const PagedAttnArgs& a, int b) {
   return r;
 }
 
+// A range that begins in no row: offsets that count packed rows many times can
+// carry the sums past 32 bits (they are reported as they are read).
+constexpr int kNoRow = -2;
+
 // `work` units (pages) cut into ranges of at least kMinUnits, as equal as can
 // be; the caller's checks keep work below 2^31.
 struct Cut {
@@ -456,10 +460,12 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
     const Cut cut(work);
     if (warp_id < kTeams) {
       const int off = range0 + warp_id < cut.ranges ? cut.start(range0 + warp_id) - (upto - own) : -1;
-      if (off >= 0 && off < own) {
+      const bool here = off >= 0 && off < own;
+      if (here) {
         const int row = off / units;
         shared->team[warp_id].start = {lane, row / tiles, row % tiles * pack, off - row * units};
       }
+      if (!__any_sync(0xffffffffu, here) && lane == 0) shared->team[warp_id].start.b = kNoRow;
     }
   } else {
     const int per = (args.batch + kThreads - 1) / kThreads;
@@ -482,6 +488,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
       if (lane >= o) before += y;
     }
     if (lane == 31) shared->scan[warp_id] = before;
+    if (threadIdx.x < kTeams) shared->team[threadIdx.x].start.b = kNoRow;
     before -= own;
     __syncthreads();
     work = 0;
@@ -522,7 +529,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
   float* sums = reinterpret_cast<float*>(smem + kTeams * kPairs * kRingBytes + team * kSumBytes);
   const Cut cut(work);
   const int range = range0 + team;
-  const bool idle = range >= cut.ranges || work == 0;
+  const bool idle = range >= cut.ranges || work == 0 || sm->start.b == kNoRow;
   volatile int* abort_flag = &sm->abort_flag;
 
   if (producer) {

@@ -652,6 +652,25 @@ def test_bad_lengths_are_reported_and_stay_in_bounds():
             ops.check_status(DEV)
 
 
+def test_offsets_that_count_rows_many_times_are_reported():
+    """Offsets that go back and forth over the packed rows, so that the scheduled pages
+    pass 32 bits; every single request is within the limits."""
+    N, G, blocks = 8193, 8, 16380
+    codes, scales, _ = make_cache([64], G, 1)
+    cu = []
+    for _ in range(4 * 289 // 2):
+        cu += [0, N - 1]
+    batch = len(cu)
+    cu.append(0)
+    q = torch.zeros(N, G, 128, dtype=torch.bfloat16, device=DEV)
+    table = torch.full((batch, blocks), -1, dtype=torch.int32, device=DEV)
+    ops.paged_attn(q, codes[0].to(DEV), codes[1].to(DEV), scales[0].to(DEV), scales[1].to(DEV),
+                   table, i32([blocks * PAGE] * batch), i32(cu), 1, blocks * PAGE)
+    with pytest.raises(_native.LeanSelectError, match="SEQLENS"):
+        ops.check_status(DEV)
+    run_attend(8, 2, [70], [1])
+
+
 def test_equal_calls_give_equal_bits_and_other_types_are_cast():
     a = run_attend(32, 2, [5000, 3], [1, 1], seed=9)
     b = run_attend(32, 2, [5000, 3], [1, 1], seed=9)
