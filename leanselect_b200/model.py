@@ -252,6 +252,8 @@ class PrefillModel:
         new = [1] * cache.batch if new_lens is None else [int(n) for n in new_lens]
         if sum(new) != input_ids.numel():
             raise ValueError("input_ids must hold sum(new_lens) tokens")
+        if not sum(new):
+            raise ValueError("decode needs new tokens")
         if not cache.max_seqlen:
             raise ValueError("decode continues a cache that prefill has filled")
         plan = cache.plan(new)

@@ -962,6 +962,8 @@ def test_model_decode_refusals(model):
         model.prefill(ids, i32([0, 64]), [64], cache=cache)
     with pytest.raises(ValueError, match="sum"):
         model.decode(ids[:2], cache)
+    with pytest.raises(ValueError, match="new tokens"):
+        model.decode(ids[:0], cache, [0])
     with pytest.raises(ValueError, match="tokens"):
         model.decode(ids[:2], cache, [2])
     with pytest.raises(RuntimeError, match="out of pages"):
