@@ -11,6 +11,7 @@ the device and running out of pages is an error on the host.
 """
 from __future__ import annotations
 
+from contextlib import contextmanager
 from typing import Sequence
 
 import torch
@@ -83,6 +84,21 @@ class PagedKVCache:
         self.seq_lens, self.free_head = plan.seq_lens, plan.free_head
         self.lengths, self.taken = after, taken
         return plan
+
+    @contextmanager
+    def step(self, new_lens: Sequence[int]):
+        """:meth:`plan` for a step that may fail on its way through the layers.
+
+        When the block raises, the cache holds the tokens it held before (rows
+        already written lie behind its lengths, and the next plan takes the
+        same pages).
+        """
+        before = self.seq_lens, self.free_head, self.lengths, self.taken, self.rope_len
+        try:
+            yield self.plan(new_lens)
+        except BaseException:
+            self.seq_lens, self.free_head, self.lengths, self.taken, self.rope_len = before
+            raise
 
     def release(self, request: int) -> None:
         """Forget a request: its pages go back to the free list."""

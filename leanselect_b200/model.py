@@ -18,6 +18,7 @@ the real checkpoint are likewise replaced by a seeded monotone ramp.
 from __future__ import annotations
 
 import math
+from contextlib import nullcontext
 from dataclasses import dataclass, field
 from typing import Callable, Sequence
 
@@ -205,35 +206,36 @@ class PrefillModel:
         """
         s = self.shape
         lengths = [int(n) for n in lengths]
-        plan = None
-        if cache is not None:
-            if cache.max_seqlen:
-                raise ValueError("prefill fills an empty cache")
-            plan = cache.plan(lengths)
-            # The frequencies its keys are rotated by; decode keeps to them.
-            cache.rope_len = max(lengths)
-        positions = (plan.positions if plan is not None else
-                     torch.cat([torch.arange(n, device=self.device) for n in lengths]))
-        freqs = self.rope.frequencies(max(lengths))
-        h = self.embed[input_ids] * s.scale_emb
-        max_len = max(lengths)
-        for i, layer in enumerate(self.layers):
-            q, k, v = self.qkv(layer, h, positions, freqs)
-            if plan is not None:
-                ops.append_kv(k, v, plan, *cache.layer(i))
-            attn, idx = prefill_layer_attention(q, k, v, cu_seqlens, max_len, layer.selector,
-                                                s.sparse, lengths=lengths, return_topk=True,
-                                                timers=timers)
-            if key_counts is not None:
-                key_counts.append(count_attended_keys(idx, lengths, s.sparse.block_size))
-            if capture is not None and layer is self.layers[-1]:
-                capture.update(q=q, k=k, v=v, idx=idx, cu=cu_seqlens, max_len=max_len)
-            del q, k, v, idx
-            h.addmm_(attn.view(h.shape[0], -1), layer.w_o.t(), alpha=self.residual_scale)
-            del attn
-            self.mlp_residual(layer, h)
-        last = cu_seqlens[1:].long() - 1
-        return self.logits(h[last])
+        if sum(lengths) != input_ids.numel():
+            raise ValueError("input_ids must hold sum(lengths) tokens")
+        if cache is not None and cache.max_seqlen:
+            raise ValueError("prefill fills an empty cache")
+        with cache.step(lengths) if cache is not None else nullcontext() as plan:
+            if cache is not None:
+                # The frequencies its keys are rotated by; decode keeps to them.
+                cache.rope_len = max(lengths)
+            positions = (plan.positions if plan is not None else
+                         torch.cat([torch.arange(n, device=self.device) for n in lengths]))
+            freqs = self.rope.frequencies(max(lengths))
+            h = self.embed[input_ids] * s.scale_emb
+            max_len = max(lengths)
+            for i, layer in enumerate(self.layers):
+                q, k, v = self.qkv(layer, h, positions, freqs)
+                if plan is not None:
+                    ops.append_kv(k, v, plan, *cache.layer(i))
+                attn, idx = prefill_layer_attention(q, k, v, cu_seqlens, max_len, layer.selector,
+                                                    s.sparse, lengths=lengths, return_topk=True,
+                                                    timers=timers)
+                if key_counts is not None:
+                    key_counts.append(count_attended_keys(idx, lengths, s.sparse.block_size))
+                if capture is not None and layer is self.layers[-1]:
+                    capture.update(q=q, k=k, v=v, idx=idx, cu=cu_seqlens, max_len=max_len)
+                del q, k, v, idx
+                h.addmm_(attn.view(h.shape[0], -1), layer.w_o.t(), alpha=self.residual_scale)
+                del attn
+                self.mlp_residual(layer, h)
+            last = cu_seqlens[1:].long() - 1
+            return self.logits(h[last])
 
     # -- decode over the 8-bit cache ---------------------------------------------------
 
@@ -256,15 +258,16 @@ class PrefillModel:
             raise ValueError("decode needs new tokens")
         if not cache.max_seqlen:
             raise ValueError("decode continues a cache that prefill has filled")
-        plan = cache.plan(new)
-        freqs = self.rope.frequencies(cache.rope_len)
-        h = self.embed[input_ids] * s.scale_emb
-        for i, layer in enumerate(self.layers):
-            q, k, v = self.qkv(layer, h, plan.positions, freqs)
-            ops.append_kv(k, v, plan, *cache.layer(i))
-            lists = page_lists(i, q) if page_lists is not None else None
-            attn = ops.paged_attn(q, *cache.layer(i), cache.block_table, plan.seq_lens,
-                                  plan.cu_seqlens_q, max(new), cache.max_seqlen, topk_idx=lists)
-            h.addmm_(attn.view(h.shape[0], -1), layer.w_o.t(), alpha=self.residual_scale)
-            self.mlp_residual(layer, h)
-        return self.logits(h)
+        with cache.step(new) as plan:
+            freqs = self.rope.frequencies(cache.rope_len)
+            h = self.embed[input_ids] * s.scale_emb
+            for i, layer in enumerate(self.layers):
+                q, k, v = self.qkv(layer, h, plan.positions, freqs)
+                ops.append_kv(k, v, plan, *cache.layer(i))
+                lists = page_lists(i, q) if page_lists is not None else None
+                attn = ops.paged_attn(q, *cache.layer(i), cache.block_table, plan.seq_lens,
+                                      plan.cu_seqlens_q, max(new), cache.max_seqlen,
+                                      topk_idx=lists)
+                h.addmm_(attn.view(h.shape[0], -1), layer.w_o.t(), alpha=self.residual_scale)
+                self.mlp_residual(layer, h)
+            return self.logits(h)

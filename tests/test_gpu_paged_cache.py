@@ -969,3 +969,37 @@ def test_model_decode_refusals(model):
     with pytest.raises(RuntimeError, match="out of pages"):
         model.decode(ids[:1], cache)
     assert cache.lengths == [64] and cache.taken == 1
+
+
+def test_failed_steps_leave_the_cache_as_it_was(model):
+    """A prefill and a decode step that raise between layers, then the same steps again."""
+    from leanselect_b200 import PagedKVCache
+
+    s = model.shape
+    gen = torch.Generator().manual_seed(12)
+    lengths = [70, 128]
+    ids = torch.randint(0, s.vocab_size, (sum(lengths),), generator=gen).to(DEV)
+    cu = i32(prefix(lengths))
+    caches = [PagedKVCache(s.num_layers, 2, 192, 6, s.num_kv_heads, device=DEV) for _ in range(2)]
+    with pytest.raises(ValueError, match="sum"):
+        model.prefill(ids, cu, [70, 127], cache=caches[0])
+    shallow = PagedKVCache(1, 2, 192, 6, s.num_kv_heads, device=DEV)
+    with pytest.raises(IndexError):
+        model.prefill(ids, cu, lengths, cache=shallow)
+    for c in (caches[0], shallow):
+        assert c.lengths == [0, 0] and c.taken == 0 and c.rope_len == 0
+    toks = [model.prefill(ids, cu, lengths, cache=c).argmax(-1) for c in caches]
+    assert torch.equal(toks[0], toks[1])
+
+    def fails_in_the_second_layer(i, q):
+        if i:
+            raise RuntimeError("no lists")
+        return torch.zeros(s.num_kv_heads, 2, 1, dtype=torch.int32, device=DEV)
+
+    with pytest.raises(RuntimeError, match="no lists"):
+        model.decode(toks[0], caches[0], page_lists=fails_in_the_second_layer)
+    assert caches[0].lengths == lengths and caches[0].taken == 4
+    for _ in range(2):
+        logits = [model.decode(toks[0], c) for c in caches]
+        assert torch.equal(*logits)
+    assert torch.equal(caches[0].block_table, caches[1].block_table)
