@@ -471,8 +471,9 @@ int ls_append_kv(const uint16_t* k, const uint16_t* v, int64_t k_stride, int64_t
  * over the request's keys in pages topk_idx[g, t, :] ([G, total_q, topk]
  * block numbers of the request, < 0 empty, duplicates count once), or in all
  * its pages when topk == 0, and with causal != 0 at positions up to the row's.
- * Rows with no key output zeros (lse = +inf); rows behind the last request
- * are left as they were.  Scales are read clamped to [2^-40, 2^48].  q and
+ * Rows with no key output zeros (lse = +inf), rows that see a NaN score NaN
+ * (lse too); rows behind the last request are left as they were.  Scales are
+ * read clamped to [2^-40, 2^48].  q and
  * out [total_q, H, 128] bf16, lse [H, total_q] fp32 (nullable); scale <= 0
  * selects 128^-0.5.  Requires 1 <= H/G <= 16, topk <= LS_MAX_TOPK.
  * max_seqlen_q / max_seqlen_k bound nq and seq_lens; the work is scheduled by

@@ -178,6 +178,20 @@ __device__ __forceinline__ uint32_t f16x2_hi(uint32_t w) {
   return d;
 }
 
+// Joining the parts of a row.  A part's reference m is -inf when it has no key
+// (its sums are 0), but also when all its scores are NaN, since the maximum
+// passes over NaN: its row sum is NaN then, and times the weight 0 it makes the
+// whole row's NaN, as it has to.  So l says whether a row has keys: with one it
+// is NaN or at least the 2^-42 that the largest score leaves (2^6, over the
+// largest value scale), and 0 without.
+__device__ __forceinline__ float part_weight(float m, float m_row) {
+  return m == -INFINITY ? 0.f : ex2(m - m_row);
+}
+__device__ __forceinline__ float row_factor(float l) { return l == 0.f ? 0.f : 1.f / l; }
+__device__ __forceinline__ float row_lse(float m, float l) {
+  return l == 0.f ? INFINITY : (m + log2f(l)) * 0.69314718055994531f;
+}
+
 __device__ __forceinline__ uint4 lds128(uint32_t addr) {
   uint4 v;
   asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
@@ -958,8 +972,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
       mt0 = fmaxf(mt0, m_part[w][gq]);
       mt1 = fmaxf(mt1, m_part[w][gq + 8]);
     }
-    const float s0 = m0 == -INFINITY ? 0.f : ex2(m0 - mt0);
-    const float s1 = m1 == -INFINITY ? 0.f : ex2(m1 - mt1);
+    const float s0 = part_weight(m0, mt0), s1 = part_weight(m1, mt1);
     // float4 k of a thread's 32 dims sits at 8c + (k ^ (c, row parity)): the
     // eight lanes of a store or load phase touch eight bank groups.
     const int swz = c | ((gq & 1) << 2);
@@ -981,7 +994,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
       for (int w = 0; w < kWarps; ++w) mt = fmaxf(mt, m_part[w][row]);
 #pragma unroll
       for (int w = 0; w < kWarps; ++w)
-        lt += m_part[w][row] == -INFINITY ? 0.f : l_part[w][row] * ex2(m_part[w][row] - mt);
+        lt = fmaf(l_part[w][row], part_weight(m_part[w][row], mt), lt);
       if (row < (kShared ? Hg * tokens : Hg)) {
         float4 sum[4];
         const int rswz = (seg >> 1) | ((row & 1) << 2);
@@ -1006,7 +1019,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
         } else {
           const int h = group * Hg + (kShared ? row % Hg : row);
           const int t = token + (kShared ? row / Hg : 0);
-          const float f = mt == -INFINITY ? 0.f : 1.f / lt;
+          const float f = row_factor(lt);
           uint4 packed[2];
           uint32_t* pw = reinterpret_cast<uint32_t*>(packed);
 #pragma unroll
@@ -1019,8 +1032,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
           dst[0] = packed[0];
           dst[1] = packed[1];
           if (args.lse != nullptr && seg == 0)
-            args.lse[static_cast<int64_t>(h) * args.total_q + t] =
-                mt == -INFINITY ? INFINITY : (mt + log2f(lt)) * 0.69314718055994531f;
+            args.lse[static_cast<int64_t>(h) * args.total_q + t] = row_lse(mt, lt);
         }
       }
     }
@@ -1052,7 +1064,7 @@ __device__ __forceinline__ float4 load_part(const float* p) {
 // heads): lane l holds its dims 4l .. 4l + 3.
 __device__ __forceinline__ void write_row(const PagedAttnArgs& args, int row, int head, int lane,
                                           float4 o, float m, float l) {
-  const float f = m == -INFINITY ? 0.f : 1.f / l;
+  const float f = row_factor(l);
   const int heads = args.heads_per_group;
   const int64_t token = row / args.num_groups + head / heads;
   const int h = (row % args.num_groups) * heads + head % heads;
@@ -1061,8 +1073,7 @@ __device__ __forceinline__ void write_row(const PagedAttnArgs& args, int row, in
   packed.y = pack_bf16x2(o.z * f, o.w * f);
   reinterpret_cast<uint2*>(args.out + (token * args.num_heads + h) * 128)[lane] = packed;
   if (args.lse != nullptr && lane == 0)
-    args.lse[static_cast<int64_t>(h) * args.total_q + token] =
-        m == -INFINITY ? INFINITY : (m + log2f(l)) * 0.69314718055994531f;
+    args.lse[static_cast<int64_t>(h) * args.total_q + token] = row_lse(m, l);
 }
 
 // The rows cut by range borders.  A row that range j begins and does not
@@ -1120,9 +1131,9 @@ __global__ void __launch_bounds__(32 * kMergeWarps) paged_merge_many_kernel(
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < kMergeWarps; ++w) m = fmaxf(m, warp_m[w]);
-  const float mine = ml.x == -INFINITY ? 0.f : ex2(ml.x - m);
+  const float mine = part_weight(ml.x, m);
   if (tid >= j && tid < j + n) weight[tid - j] = mine;
-  float l = ml.x == -INFINITY ? 0.f : ml.y * mine;
+  float l = ml.y * mine;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
   if (lane == 0) warp_l[warp] = l;
@@ -1183,14 +1194,13 @@ __global__ void __launch_bounds__(256) paged_merge_few_kernel(
     const uint32_t ends = __ballot_sync(0xffffffffu, base + lane > 0 && ends_row != 0);
     more = ends == 0;
     const int n = min(more ? 32 : __ffs(ends), ranges - j - base);
-    if (lane >= n) ml.x = -INFINITY;
+    if (lane >= n) ml = make_float2(-INFINITY, 0.f);
     float mx = fmaxf(m, ml.x);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-    const float keep = m == -INFINITY ? 0.f : ex2(m - mx);
-    const float w = ml.x == -INFINITY ? 0.f : ex2(ml.x - mx);
+    const float keep = part_weight(m, mx), w = part_weight(ml.x, mx);
     m = mx;
-    l = fmaf(l, keep, ml.x == -INFINITY ? 0.f : ml.y * w);  // a lane's share; summed at the end
+    l = fmaf(l, keep, ml.y * w);  // a lane's share; summed at the end
     acc = make_float4(acc.x * keep, acc.y * keep, acc.z * keep, acc.w * keep);
     for (int i = 0; i < n; i += 4) {
       float4 x[4];

@@ -624,6 +624,65 @@ def test_nan_and_bad_pages_in_joined_lists():
         ops.check_status(DEV)
 
 
+def nan_case(H, G, seq, nq, *, idx=None, nan_keys=(), nan_rows=(), seed=5):
+    """Output, lse and the oracle's for a cache with NaN keys ``(request, first, last + 1)``
+    and NaN query rows; where they are NaN and where a row has no key must agree."""
+    codes, scales, table = make_cache(seq, G, seed)
+    raw = codes[0].view(torch.uint8)
+    for b, first, end in nan_keys:
+        for p in range(first, end):
+            raw[table[b][p // PAGE], :, p % PAGE] = 0x7F
+    gen = torch.Generator().manual_seed(seed)
+    q = torch.randn(sum(nq), H, 128, generator=gen).bfloat16()
+    for t in nan_rows:
+        q[t, 0] = math.nan
+    got, lse = ops.paged_attn(
+        q.to(DEV), codes[0].to(DEV), codes[1].to(DEV), scales[0].to(DEV), scales[1].to(DEV),
+        i32(table), i32(seq), i32(prefix(nq)), max(nq), max(seq),
+        topk_idx=None if idx is None else idx.to(DEV), return_lse=True)
+    want, want_lse, bounds = ora.attend(q, codes[0].float(), codes[1].float(), scales[0], scales[1],
+                                        table, seq, prefix(nq), idx)
+    got, lse = got.double().cpu(), lse.double().cpu()
+    assert bool(want_lse.isnan().any())
+    assert torch.equal(got.isnan(), want.isnan())
+    assert torch.equal(lse.isnan(), want_lse.isnan())
+    assert torch.equal(lse.isinf(), want_lse.isinf())
+    ok, fine = ~want.isnan(), torch.isfinite(want_lse)
+    assert bool(((got - want).abs()[ok] <= tolerance(want, bounds, max(seq))[ok]).all())
+    d = 128 * 2.0 ** -23 * bounds[1].T + 2.0 ** -20
+    ltol = d + max(seq) * 2.0 ** -24 + 2.0 ** -22 * (want_lse.abs() + 64)
+    assert bool(((lse - want_lse).abs()[fine] <= ltol[fine]).all())
+
+
+@pytest.mark.parametrize("H, G, seq, nq", [
+    (16, 1, [1, 70, 0], [1, 1, 1]),          # rows inside one range
+    (8, 2, [5000], [1]),                     # one row in many parts: joined by row
+    (8, 1, [3000] * 24, [1] * 24),           # rows of a few parts: joined by range
+    (4, 1, [300, 5], [5, 2]),                # several tokens a tile
+    (4, 1, [2600] * 8, [4] * 8),             # and tiles cut by range borders
+])
+def test_lse_of_nan_scores_is_nan(H, G, seq, nq):
+    """Every key of a warp's share, of a page, of a row, or the query itself is NaN: the
+    row's lse is NaN, never finite and never the +inf of a row without keys."""
+    last = seq[0]
+    for first, end in ((0, 1), (0, min(last, 32)), (0, min(last, 64)), (last - 1, last), (0, last)):
+        nan_case(H, G, seq, nq, nan_keys=[(0, first, end)])
+    nan_case(H, G, seq, nq, nan_rows=[0])
+
+
+@pytest.mark.parametrize("H, n", [(16, 3), (4, 3), (4, 1200)])
+def test_lse_of_nan_scores_in_listed_pages(H, n):
+    """As above where rows list their pages: alone, and (1200 rows of 4 heads) joined."""
+    T = 128 if n > 3 else 3
+    idx = torch.full((1, n, T), -1, dtype=torch.int32)
+    for i in range(n):
+        pages = ([0], [1, 2], [0, 2], [])[i % 4]
+        idx[0, i, :len(pages)] = torch.tensor(pages, dtype=torch.int32)
+    seq = [max(190, n)]
+    nan_case(H, 1, seq, [n], idx=idx, nan_keys=[(0, 0, 64)])
+    nan_case(H, 1, seq, [n], idx=idx, nan_rows=[1, n - 2])
+
+
 def test_bad_pages_are_passed_over_and_reported():
     codes, scales, table = make_cache([300, 64], 2, 3)
     table[0][1] = 10 ** 6
