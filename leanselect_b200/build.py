@@ -28,7 +28,7 @@ BINDING_STAMP = LIB_DIR / "_binding.torch"
 BINDING_SOURCE = CSRC / "binding.cpp"
 SOURCES = ["prep.cu", "score_select.cu", "sparse_attn.cu", "capi.cu", "backbone.cu", "noalloc.cu",
            "waitprobe.cu", "select_f32.cu", "paged_cache.cu", "paged_attn.cu"]
-HEADERS = ["common.cuh", "launch.h", "topk_rows.cuh", "page_list.cuh"]
+HEADERS = ["common.cuh", "launch.h", "topk_rows.cuh", "page_list.cuh", "paged_schedule.h"]
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr",

@@ -855,6 +855,9 @@ int ls_paged_attn(const uint16_t* q, const uint8_t* k_pages, const uint8_t* v_pa
   LS_REQUIRE(workspace && workspace_bytes >= need, "workspace too small: %zu < %zu bytes",
              workspace_bytes, need);
   LS_REQUIRE_ALIGNED(workspace);
+  const PagedSizes sizes{total_q, batch,      num_kv_heads, hg,
+                         topk,    max_blocks, max_seqlen_q, max_seqlen_k};
+  LS_REQUIRE(paged_rows_fit(sizes), "total_q * num_kv_heads * pages per row out of range");
   int device = 0, sms = 0;
   cudaError_t err = cudaGetDevice(&device);
   if (err == cudaSuccess)
@@ -890,34 +893,10 @@ int ls_paged_attn(const uint16_t* q, const uint8_t* k_pages, const uint8_t* v_pa
   a.part_ml = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kPagedMaxRanges * 16);
   a.part_o = a.part_ml + 2 * kPagedMaxRanges * 16 * 2;
   a.status = status;
-  // At most one range per scheduled page: the caller's max_seqlen_k bounds the
-  // pages of a dense row (a longer request only gets fewer ranges).
-  LS_REQUIRE(total_q * num_kv_heads * ((topk > 0 ? topk : max_blocks) + kPagedRowCost) <
-                 (int64_t{1} << 31),
-             "total_q * num_kv_heads * pages per row out of range");
-  const int64_t most_pages = std::max<int64_t>(1, (int64_t{max_seqlen_k} + 63) / 64);
-  a.units = static_cast<int>(topk > 0 ? std::min<int64_t>(topk, most_pages) : 0);
-  // A tile of 16 rows takes as many tokens of a request as their heads fit, so
-  // that a draft or a chunk reads each page once for all of them: 8 tokens over
-  // 131072 keys, 2 x 8 heads, take 55 us against 87 one by one.  Page lists are
-  // joined for that where a table of the request's pages fits on chip, where
-  // they must overlap threefold (one visit for several tokens masks per page
-  // and costs twice as much: 512 tokens of 2 x 2 heads with 96 of 256 pages
-  // each 156 us against 204, with 96 of 384 pages 220 against 212) and where 30
-  // pages per range, rows' own cost included, hide the joining (512 tokens of 2
-  // x 4 heads over 5 pages 19 us against 27; 128 of 2 x 1 heads with 16 of 16
-  // pages 20 against 18, 32 of 2 x 4 with 32 of 42 pages 19 against 14).
-  a.pack = 1;
-  if (max_seqlen_q > 1) {
-    const int tokens = std::min(16 / hg, static_cast<int>(max_seqlen_q));
-    if (topk == 0 || (most_pages <= kPagedMaxUnion && int64_t{tokens} * a.units >= 3 * most_pages &&
-                      total_q * num_kv_heads * (a.units + kPagedRowCost) >= int64_t{30} * 2 * sms))
-      a.pack = tokens;
-  }
-  const int64_t per_row = topk > 0 ? a.units : most_pages;
-  const int64_t want = total_q * num_kv_heads * per_row;
-  const int ranges = static_cast<int>(std::min<int64_t>({want, 2 * sms, kPagedMaxRanges}));
-  err = launch_paged_attn(a, ranges, static_cast<cudaStream_t>(stream));
+  const PagedSchedule schedule = paged_schedule(sizes, sms);
+  a.units = schedule.units;
+  a.pack = schedule.pack;
+  err = launch_paged_attn(a, schedule.ranges, static_cast<cudaStream_t>(stream));
   return err == cudaSuccess ? LS_OK : cuda_fail(err, "paged_attn launch");
 }
 

@@ -5,6 +5,8 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
+#include "paged_schedule.h"
+
 namespace ls {
 
 cudaError_t launch_fold_weights(const float* head_mix, const float* kv_head_mix,
@@ -190,13 +192,6 @@ struct AppendArgs {
 cudaError_t launch_append_kv(const AppendArgs& args, cudaStream_t stream);
 
 // Attention over the paged cache (paged_attn.cu).
-constexpr int kPagedMaxRanges = 2 * 148;  // work ranges: two on each of the B200's SMs
-
-// Units of work a row counts for besides its pages.
-constexpr int kPagedRowCost = 4;
-// Most pages of a request whose tokens' page lists are joined in one tile.
-constexpr int kPagedMaxUnion = 512;
-
 struct PagedAttnArgs {
   CUtensorMap tm_k;       // K codes as [num_pages * G * 64, 128] bytes, box {128, 64}, 128B swizzle
   CUtensorMap tm_v;

@@ -399,7 +399,7 @@ __device__ __forceinline__ Request load_request(const PagedAttnArgs& a, int b) {
 constexpr int kNoRow = -2;
 
 // `work` units (pages) cut into ranges of at least kMinUnits, as equal as can
-// be; the caller's checks keep work below 2^31.
+// be; paged_schedule.h keeps work below 2^31.
 struct Cut {
   int ranges, size, longer;  // `longer` ranges have one unit more
   __device__ __forceinline__ Cut(int work) {

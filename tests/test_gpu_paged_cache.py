@@ -730,6 +730,42 @@ def test_offsets_that_count_rows_many_times_are_reported():
     run_attend(8, 2, [70], [1])
 
 
+def test_lists_of_very_many_requests():
+    """One token each of 140000 requests of 512 pages, 32 heads, lists long enough to be
+    joined: rows alone are within 32 bits of work, tiles of joined lists would not be."""
+    N, H, T = 140000, 32, 96
+    codes, scales, _ = make_cache([64], H, 1, nan_tail=False)
+    cache = [codes[0].to(DEV), codes[1].to(DEV), scales[0].to(DEV), scales[1].to(DEV)]
+    gen = torch.Generator(device=DEV).manual_seed(1)
+    q = torch.randn(N, H, 128, generator=gen, device=DEV, dtype=torch.bfloat16)
+    idx = torch.full((H, N, T), -1, dtype=torch.int32, device=DEV)
+    idx[..., 0] = 500
+    out = torch.full_like(q, math.nan)
+    # all blocks are page 0, of 512 x 64 tokens the row lists one page
+    _, lse = ops.paged_attn(q, *cache, torch.zeros(N, 512, dtype=torch.int32, device=DEV),
+                            torch.full((N,), 512 * 64, dtype=torch.int32, device=DEV),
+                            torch.arange(N + 1, dtype=torch.int32, device=DEV), 16, 512 * 64,
+                            topk_idx=idx, return_lse=True, out=out)
+    del idx
+    k, v = (c[0].double() * s[0].double()[:, None, None] for c, s in ((cache[0], cache[2]),
+                                                                     (cache[1], cache[3])))
+    for t in range(0, N, 10000):
+        qr = q[t:t + 10000].double()
+        x = torch.einsum("thd,hkd->thk", qr, k) / math.sqrt(128)
+        w = torch.softmax(x, -1)
+        sv = cache[3][0].double()
+        bounds = (torch.einsum("thk,hkd->thd", w, v.abs()),
+                  torch.einsum("thd,hkd->thk", qr.abs(), k.abs()).amax(-1) / math.sqrt(128),
+                  (w.amax(-1) * sv)[..., None] * (v.abs() / sv[:, None, None]).sum(1))
+        want = torch.einsum("thk,hkd->thd", w, v)
+        err = (out[t:t + 10000].double() - want).abs()
+        assert bool((err <= tolerance(want, bounds, 64)).all())
+        want = torch.logsumexp(x, -1)
+        ltol = 128 * 2.0 ** -23 * bounds[1] + 2.0 ** -20 + 64 * 2.0 ** -24 + 2.0 ** -22 * (
+            want.abs() + 64)
+        assert bool(((lse.T[t:t + 10000].double() - want).abs() <= ltol).all())
+
+
 def test_equal_calls_give_equal_bits_and_other_types_are_cast():
     a = run_attend(32, 2, [5000, 3], [1, 1], seed=9)
     b = run_attend(32, 2, [5000, 3], [1, 1], seed=9)

@@ -1,5 +1,8 @@
 """The paged cache's argument checks and its 64-bit oracle, without a GPU."""
 import ctypes
+import shutil
+import subprocess
+from pathlib import Path
 
 import pytest
 import torch
@@ -92,6 +95,60 @@ ATTEND = [FAKE, FAKE, FAKE, FAKE, FAKE, 5, FAKE, 4, FAKE, FAKE, 2, 1, 200, 2, 32
 ])
 def test_attention_refusals(changes, code, text):
     refused("ls_paged_attn", ATTEND, changes, code, text)
+
+
+SCHEDULE = r"""
+#include <cstdio>
+#include "paged_schedule.h"
+
+int main() {
+  ls::PagedSizes s;
+  long long total_q;
+  while (scanf("%lld %d %d %d %d %d %d %d", &total_q, &s.batch, &s.num_kv_heads,
+               &s.heads_per_group, &s.topk, &s.max_blocks, &s.max_seqlen_q, &s.max_seqlen_k) == 8) {
+    s.total_q = total_q;
+    const ls::PagedSchedule r = ls::paged_schedule(s, 148);
+    printf("%d %d %d %d\n", ls::paged_rows_fit(s) ? 1 : 0, r.units, r.pack, r.ranges);
+  }
+  return 0;
+}
+"""
+
+
+@pytest.mark.skipif(shutil.which("g++") is None, reason="no C++ compiler")
+def test_scheduled_work_stays_within_32_bits(tmp_path):
+    """Every call the range check lets through gives the kernels less than 2^31 units,
+    whatever way the tokens are dealt to the requests."""
+    root = Path(__file__).resolve().parents[1]
+    src, exe = tmp_path / "schedule.cpp", tmp_path / "schedule"
+    src.write_text(SCHEDULE)
+    subprocess.run(["g++", "-std=c++17", "-Wall", "-Wextra", "-Werror", "-I",
+                    str(root / "leanselect_b200" / "csrc"), str(src), "-o", str(exe)], check=True)
+    cases = [(n, b, G, hg, topk, blocks, mq, 64 * min(blocks, 512))
+             for hg in (1, 3, 8, 16) for topk in (0, 1, 96, 128) for blocks in (1, 40, 512, 2048)
+             for mq in (1, 2, 16, 1000) for G in (1, 32)
+             for n, b in ((1, 1), (2000, 1), (140000, 140000), (140000, 1000), (4200000, 4199985),
+                          (16000000, 16000000), (1 << 26, 3))]
+    text = "\n".join(" ".join(map(str, c)) for c in cases)
+    out = subprocess.run([str(exe)], input=text, capture_output=True, text=True, check=True).stdout
+    joined = alone = 0
+    for (n, b, G, hg, topk, blocks, mq, mk), line in zip(cases, out.splitlines(), strict=True):
+        fits, units, pack, ranges = map(int, line.split())
+        assert bool(fits) == (n * G * ((topk or blocks) + 4) < 1 << 31)
+        if not fits:
+            continue
+        assert 1 <= ranges <= 296 and 1 <= pack <= max(1, min(16 // hg, mq))
+        # requests of a token each and one of the rest; and tokens dealt evenly
+        for lens in ([(b - 1, 1), (1, n - b + 1)], [(b - n % b, n // b), (n % b, n // b + 1)]):
+            tiles = sum(count * -(-m // pack) for count, m in lens)
+            if topk and pack == 1:
+                work = n * G * (units + 4)
+            else:
+                work = tiles * G * (min(pack * topk, blocks) + 4 if topk else blocks + 4)
+            assert work < 1 << 31, (n, b, G, hg, topk, blocks, mq)
+        joined += bool(topk) and pack > 1
+        alone += (n, b, G, hg, topk, blocks, mq) == (140000, 140000, 32, 1, 96, 512, 16) and pack == 1
+    assert joined > 20 and alone == 1
 
 
 def test_attention_of_no_rows_is_ok():
