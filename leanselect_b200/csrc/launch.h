@@ -1,6 +1,7 @@
 // Internal launcher declarations shared by the kernels and the C ABI layer.
 #pragma once
 
+#include <atomic>
 #include <cstdint>
 #include <cuda.h>
 #include <cuda_runtime.h>
@@ -127,6 +128,21 @@ cudaError_t launch_sparse_attn_merge(const AttnArgs& args, cudaStream_t stream);
 // nothing is written.  Its duration is the L2 -> shared-memory gather time
 // the attention kernel cannot beat (a measured roofline for it).
 cudaError_t launch_sparse_attn_gather_only(const AttnArgs& args, cudaStream_t stream);
+
+// Runs `prepare` (kernel attributes) once per device, whichever thread calls
+// first; again if it failed.  `done` is a bit per device, set once it is ready.
+template <typename F>
+cudaError_t once_per_device(std::atomic<uint64_t> (&done)[4], F prepare) {
+  int device = 0;
+  cudaError_t err = cudaGetDevice(&device);
+  if (err != cudaSuccess) return err;
+  const uint64_t bit = uint64_t{1} << (device & 63);
+  const bool tracked = device >= 0 && device < 256;
+  if (tracked && (done[device >> 6].load(std::memory_order_acquire) & bit)) return cudaSuccess;
+  err = prepare();
+  if (err == cudaSuccess && tracked) done[device >> 6].fetch_or(bit, std::memory_order_release);
+  return err;
+}
 
 // Launches a kernel that may be set up while the stream's previous kernel
 // still runs; the kernel calls wait_for_inputs() before it touches memory.

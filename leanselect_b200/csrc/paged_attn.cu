@@ -46,8 +46,6 @@
 // bookkeeping), keep the tensor pipe 40 % busy.  Tried and dropped there: three teams
 // at 152 registers (152 us, but 5 us more for one long request), the next
 // page's scores formed beside this page's product with V (168-186 us).
-#include <atomic>
-
 #include <cuda_fp16.h>
 
 #include "common.cuh"
@@ -1228,22 +1226,16 @@ __global__ void __launch_bounds__(256) paged_merge_few_kernel(
 // shared memory limit.
 template <bool kHalf, bool kShared>
 cudaError_t prepare_attn_kernel() {
-  static std::atomic<uint64_t> ready[4];  // a bit per device, set once it is done there
-  int device = 0;
-  cudaError_t err = cudaGetDevice(&device);
-  if (err != cudaSuccess) return err;
-  const uint64_t bit = uint64_t{1} << (device & 63);
-  const bool tracked = device >= 0 && device < 256;
-  if (tracked && (ready[device >> 6].load(std::memory_order_acquire) & bit)) return cudaSuccess;
-  cudaFuncAttributes attr;
-  err = cudaFuncGetAttributes(&attr, paged_attn_kernel<kHalf, kShared>);
-  if (err != cudaSuccess) return err;
-  if (attr.numRegs != kLaunchRegs) return cudaErrorInvalidConfiguration;
-  err = cudaFuncSetAttribute(paged_attn_kernel<kHalf, kShared>,
-                             cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             static_cast<int>(paged_smem_bytes()));
-  if (err == cudaSuccess && tracked) ready[device >> 6].fetch_or(bit, std::memory_order_release);
-  return err;
+  static std::atomic<uint64_t> done[4];
+  return once_per_device(done, [] {
+    cudaFuncAttributes attr;
+    const cudaError_t err = cudaFuncGetAttributes(&attr, paged_attn_kernel<kHalf, kShared>);
+    if (err != cudaSuccess) return err;
+    if (attr.numRegs != kLaunchRegs) return cudaErrorInvalidConfiguration;
+    return cudaFuncSetAttribute(paged_attn_kernel<kHalf, kShared>,
+                                cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                static_cast<int>(paged_smem_bytes()));
+  });
 }
 
 template <bool kHalf, bool kShared>

@@ -414,16 +414,20 @@ __global__ void __launch_bounds__(2 * kThreads, kThreads == 128 ? 3 : 16) append
 }  // namespace
 
 cudaError_t launch_plan_pages(const PlanArgs& args, cudaStream_t stream) {
-  const size_t smem = 2 * sizeof(int32_t) * (static_cast<size_t>(args.batch) + 1);
-  if (smem > 40 * 1024) {
-    const cudaError_t err =
-        cudaFuncSetAttribute(plan_pages_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             static_cast<int>(smem));
-    if (err != cudaSuccess) return err;
-  }
+  const auto smem_bytes = [](int batch) {
+    return 2 * sizeof(int32_t) * (static_cast<size_t>(batch) + 1);
+  };
+  // Set once, to what the largest batch takes: calls of other threads rely on it.
+  static std::atomic<uint64_t> done[4];
+  const cudaError_t err = once_per_device(done, [&] {
+    return cudaFuncSetAttribute(plan_pages_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                static_cast<int>(smem_bytes(LS_MAX_PLAN_BATCH)));
+  });
+  if (err != cudaSuccess) return err;
   const int64_t want = (args.total_new + kPlanThreads - 1) / kPlanThreads;
   const unsigned grid = static_cast<unsigned>(want < 1 ? 1 : want > 148 * 4 ? 148 * 4 : want);
-  return launch_early(plan_pages_kernel, dim3(grid), dim3(kPlanThreads), smem, stream, args);
+  return launch_early(plan_pages_kernel, dim3(grid), dim3(kPlanThreads), smem_bytes(args.batch),
+                      stream, args);
 }
 
 cudaError_t launch_append_kv(const AppendArgs& args, cudaStream_t stream) {

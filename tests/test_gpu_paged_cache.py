@@ -21,7 +21,11 @@ Tolerances:
 * log-sum-exp: d + N 2^-24 for the sum, and 2^-22 (|ref| + 64) for the
   roundings of the reference exponent.
 """
+import ctypes
 import math
+import shutil
+import subprocess
+from pathlib import Path
 
 import pytest
 import torch
@@ -158,6 +162,67 @@ def test_plan_bad_lengths_are_reported(context, new, total):
         assert slots[1 + 6:] == [-1] * 14 and slots[1] == 7 * 64 + 58
     with pytest.raises(_native.LeanSelectError, match="SEQLENS"):
         ops.check_status(DEV)
+
+
+PLAN_THREADS = r"""
+#include <atomic>
+#include <thread>
+#include <vector>
+#include "leanselect_b200.h"
+
+// Plans of `calls` steps each from `count` threads that start together; the
+// first failing code, or 0.
+extern "C" int run(int count, int calls, const int32_t* batch, int32_t* const* ctx,
+                   int32_t* const* add, int32_t* const* table, int32_t* const* out,
+                   int32_t* const* head, int32_t* status, void* const* stream) {
+  std::atomic<int> waiting(count), failed(0);
+  std::vector<std::thread> threads;
+  for (int i = 0; i < count; ++i)
+    threads.emplace_back([&, i] {
+      const int b = batch[i];
+      for (--waiting; waiting.load() > 0;) {}
+      for (int k = 0; k < calls; ++k) {
+        const int rc = ls_plan_pages(ctx[i], add[i], b, table[i], 2, nullptr, 0, head[i], 0, out[i],
+                                     out[i] + b, out[i] + 2 * b + 1, nullptr, nullptr,
+                                     head[i] + 1, status, stream[i]);
+        int none = 0;
+        if (rc != LS_OK) failed.compare_exchange_strong(none, rc);
+      }
+    });
+  for (auto& t : threads) t.join();
+  return failed.load();
+}
+"""
+
+
+@pytest.mark.skipif(shutil.which("g++") is None, reason="no C++ compiler")
+def test_plans_from_several_threads(tmp_path):
+    """Batches whose plans need different amounts of shared memory, planned at once."""
+    lib = Path(_native.load()._name)
+    src, so = tmp_path / "threads.cpp", tmp_path / "threads.so"
+    src.write_text(PLAN_THREADS)
+    include = Path(__file__).resolve().parents[1] / "include"
+    subprocess.run(["g++", "-std=c++17", "-O1", "-shared", "-fPIC", "-pthread", "-I", str(include),
+                    str(src), "-o", str(so), str(lib), f"-Wl,-rpath,{lib.parent}"], check=True)
+    batches = [5200, 6100, 7000, 8192, 40]
+    tensors = [[i32([63] * b), i32([0] * b), i32([[-1, -1]] * b),
+                torch.empty(3 * b + 2, dtype=torch.int32, device=DEV), i32([0, -1])]
+               for b in batches]
+    streams = [torch.cuda.Stream() for _ in batches]
+    torch.cuda.synchronize()
+
+    def pointers(values):
+        return (ctypes.c_void_p * len(values))(*values)
+
+    rows = [pointers([t[i].data_ptr() for t in tensors]) for i in range(5)]
+    rc = ctypes.CDLL(str(so)).run(
+        len(batches), 400, (ctypes.c_int32 * len(batches))(*batches), *rows,
+        ctypes.c_void_p(ops.status_word(DEV).data_ptr()),
+        pointers([s.cuda_stream for s in streams]))
+    torch.cuda.synchronize()
+    assert rc == 0, _native.load().ls_status_string(rc)
+    for b, t in zip(batches, tensors):
+        assert t[4].tolist() == [0, 0] and t[3][:b].tolist() == [63] * b
 
 
 def test_plan_refusals():
