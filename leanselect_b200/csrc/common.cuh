@@ -241,6 +241,15 @@ __device__ __forceinline__ void wait_for_inputs() {
   asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
+// Reads memory that the stream's previous kernels write, behind
+// wait_for_inputs().  An ordinary load: __ldg may only read what is constant for
+// the kernel's whole life, and this kernel's life begins before they have ended
+// (the compiler may even move such a load across the wait).
+template <typename T>
+__device__ __forceinline__ T load_input(const T* p) {
+  return *p;
+}
+
 // Lets the next kernel of the stream be set up once every CTA has got here; it
 // still waits for this grid's end if it was launched early, as above.
 __device__ __forceinline__ void allow_next_launch() {

@@ -238,7 +238,8 @@ __device__ __forceinline__ void load_query(const PagedAttnArgs& args, int token,
     uint4 raw[4];
     float amax = 0.f;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) raw[k] = h < heads * tokens ? __ldg(src + k) : make_uint4(0, 0, 0, 0);
+    for (int k = 0; k < 4; ++k)
+      raw[k] = h < heads * tokens ? load_input(src + k) : make_uint4(0, 0, 0, 0);
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       const uint32_t w[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
@@ -293,7 +294,7 @@ __device__ __forceinline__ int union_pages(const PagedAttnArgs& args, uint32_t* 
 #pragma unroll
     for (int r = 0; r < LS_MAX_TOPK / 32; ++r) {
       const int pos = 32 * r + lane;
-      const int32_t p = pos < args.topk ? __ldg(list + t * args.topk + pos) : -1;
+      const int32_t p = pos < args.topk ? load_input(list + t * args.topk + pos) : -1;
       bad = bad || p >= n_pages;
       if (p >= 0 && p < most && p * kPage <= limit_t) atomicOr(pages + p, 1u << t);
     }
@@ -382,14 +383,24 @@ struct Request {
 
 __device__ __forceinline__ Request load_request(const PagedAttnArgs& a, int b) {
   Request r;
-  r.q0 = __ldg(a.cu_q + b);
-  const int end = __ldg(a.cu_q + b + 1), len = __ldg(a.seq_lens + b);
+  r.q0 = load_input(a.cu_q + b);
+  const int end = load_input(a.cu_q + b + 1), len = load_input(a.seq_lens + b);
   const int most = a.max_blocks * kPage;  // at most 2^30
   const bool rows_ok = r.q0 >= 0 && end >= r.q0 && end <= a.total_q;
   r.bad = !rows_ok || len < 0 || len > most;
   r.nq = rows_ok ? end - r.q0 : 0;
   r.len = min(max(len, 0), most);
   return r;
+}
+
+// Last request whose first row is at or before `row`.
+__device__ __forceinline__ int find_request(const PagedAttnArgs& a, int row) {
+  int lo = 0, hi = a.batch - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (load_input(a.cu_q + mid) <= row) lo = mid; else hi = mid - 1;
+  }
+  return lo;
 }
 
 // A range that begins in no row: offsets that count packed rows many times can
@@ -445,7 +456,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
   const int range0 = static_cast<int>(blockIdx.x) * kTeams;
   int work, rows_listed = 0;
   if (single) {
-    rows_listed = min(max(__ldg(args.cu_q + args.batch), 0), static_cast<int>(args.total_q));
+    rows_listed = min(max(load_input(args.cu_q + args.batch), 0), static_cast<int>(args.total_q));
     const int units = args.units + kPagedRowCost;
     work = rows_listed * G * units;
     const Cut cut(work);
@@ -578,7 +589,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
       if (single) {
         token = at.token;
         if (at.b < 0 || token < req.q0 || token >= req.q0 + req.nq) {
-          at.b = find_sequence(args.cu_q, args.batch, token);
+          at.b = find_request(args, token);
           req = load_request(args, at.b);
           if (req.bad && lane == 0) report(args.status, LS_DEVERR_SEQLENS);
         }
@@ -619,7 +630,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const int pos = 32 * r + lane;
-          const int32_t p = pos < args.topk ? __ldg(list + pos) : -1;
+          const int32_t p = pos < args.topk ? load_input(list + pos) : -1;
           bad = bad || p >= n_pages;
           v[r] = (p >= 0 && p < n_pages && p * kPage <= limit) ? p : kPageSentinel;
         }
@@ -650,12 +661,12 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
           const uint32_t entry = listed ? ps->pages[i] : i;
           const int logical = listed && !single ? entry >> 16 : entry;
           if (listed && !single) mask = entry & 0xFFFF;
-          const int page = __ldg(table + logical);
+          const int page = load_input(table + logical);
           d.key0 = logical * kPage;
           if (page >= 0 && page < args.num_pages) {
             y = (page * G + g) * kPage;
-            ks = __ldg(args.k_scale + static_cast<int64_t>(page) * G + g);
-            vs = __ldg(args.v_scale + static_cast<int64_t>(page) * G + g);
+            ks = load_input(args.k_scale + static_cast<int64_t>(page) * G + g);
+            vs = load_input(args.v_scale + static_cast<int64_t>(page) * G + g);
           } else {
             report(args.status, LS_DEVERR_PAGE_INDEX);
           }

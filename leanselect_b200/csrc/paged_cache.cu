@@ -40,7 +40,7 @@ struct PlanRow {
 
 __device__ __forceinline__ PlanRow plan_row(const PlanArgs& a, int b) {
   PlanRow r;
-  const int ctx = __ldg(a.context_lens + b), n = __ldg(a.new_lens + b);
+  const int ctx = load_input(a.context_lens + b), n = load_input(a.new_lens + b);
   const int c = min(max(ctx, 0), 1 << 30), m = min(max(n, 0), 1 << 30);
   const int total = static_cast<int>((static_cast<uint32_t>(c) + m + kPage - 1) / kPage);
   r.ctx = c;
@@ -149,7 +149,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_pages_kernel(const __grid_c
     tok_run += r.n;
     blk_run += r.blocks();
   }
-  const int64_t head_in = __ldg(a.free_head);
+  const int64_t head_in = load_input(a.free_head);
   const int64_t head = min(max(head_in, int64_t{0}), static_cast<int64_t>(a.num_free));
   if (tid == 0) {
     const int64_t taken = static_cast<int64_t>(blk_all >> 32);
@@ -181,7 +181,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_pages_kernel(const __grid_c
         const int mid = (b + top + 1) >> 1;
         if (cu_q[mid] <= i) b = mid; else top = mid - 1;
       }
-      const int ctx = min(max(__ldg(a.context_lens + b), 0), 1 << 30);
+      const int ctx = min(max(load_input(a.context_lens + b), 0), 1 << 30);
       pos = ctx + (i - cu_q[b]);
       const int block = pos / kPage, had = (ctx + kPage - 1) / kPage;
       if (block < a.max_blocks) {
@@ -191,7 +191,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_pages_kernel(const __grid_c
           page = *entry;
         } else {
           const int64_t from = head + cu_need[b] + (block - had);
-          page = from < a.num_free ? __ldg(a.free_pages + from) : -1;
+          page = from < a.num_free ? load_input(a.free_pages + from) : -1;
           if (pos % kPage == 0) *entry = page;
         }
         if (page >= 0) slot = static_cast<int64_t>(page) * kPage + pos % kPage;
@@ -256,17 +256,17 @@ __device__ __forceinline__ BlockRows find_block(const AppendArgs& a, int64_t ite
     lo = static_cast<int>(min(max(item - 16, int64_t{0}), static_cast<int64_t>(n - 32)));
     n = 32;
   }
-  const int total = __ldg(a.cu_blocks + a.batch);
+  const int total = load_input(a.cu_blocks + a.batch);
   for (int round = 0; round < 2; ++round) {
     const int b = lo + lane;
     int first = 0x7FFFFFFF, ctx = 0, seq = 0, q0 = 0;
     if (lane < n) {
-      first = __ldg(a.cu_blocks + b);
-      ctx = __ldg(a.context_lens + b);
-      seq = __ldg(a.seq_lens + b);
-      q0 = __ldg(a.cu_seqlens_q + b);
+      first = load_input(a.cu_blocks + b);
+      ctx = load_input(a.context_lens + b);
+      seq = load_input(a.seq_lens + b);
+      q0 = load_input(a.cu_seqlens_q + b);
     }
-    const int behind = __ldg(a.cu_blocks + lo + n);
+    const int behind = load_input(a.cu_blocks + lo + n);
     const uint32_t at = __ballot_sync(0xffffffffu, lane < n && first <= item);
     if (item >= total) return {0, 0, 0, BlockRows::kNone};
     if (at != 0 && item < behind) {
@@ -293,7 +293,7 @@ __device__ __forceinline__ BlockRows find_block(const AppendArgs& a, int64_t ite
     while (to - from > 32) {
       const int step = (to - from + 31) / 32, probe = from + lane * step;
       const uint32_t before =
-          __ballot_sync(0xffffffffu, probe < to && __ldg(a.cu_blocks + probe) <= item);
+          __ballot_sync(0xffffffffu, probe < to && load_input(a.cu_blocks + probe) <= item);
       const int pick = before == 0 ? 0 : 31 - __clz(before);
       from += pick * step;
       to = min(from + step, to);
@@ -333,14 +333,15 @@ __global__ void __launch_bounds__(2 * kThreads, kThreads == 128 ? 3 : 16) append
     if (rows.state == BlockRows::kBad && threadIdx.x == 0) report(a.status, LS_DEVERR_SEQLENS);
     return;
   }
-  const int64_t slot = __ldg(a.slots + rows.t0);
+  const int64_t slot = load_input(a.slots + rows.t0);
   const int r0 = rows.r0, r1 = rows.r1;
   const uint16_t* src = (is_v ? a.v : a.k) + g * 128;
   const int64_t row_stride = is_v ? a.v_stride : a.k_stride;
   const int c = threadIdx.x & 15, r = (threadIdx.x % kThreads) >> 4;
   const auto load = [&](int row) {
-    return row < r1 ? __ldg(reinterpret_cast<const uint4*>(src + (rows.t0 + (row - r0)) * row_stride) + c)
-                    : make_uint4(0, 0, 0, 0);
+    if (row >= r1) return make_uint4(0, 0, 0, 0);
+    return load_input(
+        reinterpret_cast<const uint4*>(src + (rows.t0 + (row - r0)) * row_stride) + c);
   };
   // Rows r0 + r, r0 + r + kRows, ...: the first passes stay in registers, the
   // others (kThreads == 32, more than 4 new rows) are read again.

@@ -240,3 +240,16 @@ def test_custom_op_shapes():
     out, lse = registered.paged_attn(t(70, 16, 128, dtype=torch.bfloat16), *cache, t(5, 9), seq,
                                      cu_q, 30, 500, None, 0.0, True)
     assert out.shape == (70, 16, 128) and lse.shape == (16, 70) and lse.dtype == torch.float32
+
+
+def test_kernels_launched_early_read_with_ordinary_loads():
+    """Such a kernel begins while its predecessor still writes its inputs: loads that need
+    data which is constant for the kernel's life (``__ldg``, ``ld.global.nc``, and what the
+    compiler makes of const restrict pointers) must not read them."""
+    csrc = Path(__file__).resolve().parents[1] / "leanselect_b200" / "csrc"
+    early = [f for f in csrc.glob("*.cu") if "launch_early(" in f.read_text()]
+    assert {f.name for f in early} >= {"paged_attn.cu", "paged_cache.cu"}
+    for f in early:
+        text = f.read_text()
+        for bad in ("__ldg(", "__ldca(", "global.nc", "__restrict__", "find_sequence("):
+            assert bad not in text, (f.name, bad)
