@@ -653,7 +653,8 @@ def _token_rows(t: torch.Tensor) -> torch.Tensor:
     if (t.stride(2) == 1 and t.stride(1) == t.shape[2] and t.stride(0) % 8 == 0
             and t.stride(0) >= t.shape[1] * t.shape[2] and t.data_ptr() % 16 == 0):
         return t
-    return t.contiguous()
+    # Not contiguous(): it returns a single token with any stride, and any alignment, as it is.
+    return t.clone(memory_format=torch.contiguous_format)
 
 
 def append_kv(k: torch.Tensor, v: torch.Tensor, plan: PagePlan, k_pages: torch.Tensor,

@@ -373,6 +373,15 @@ def test_append_views_of_a_fused_projection_and_other_types():
     assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(cache, twin))
 
 
+def test_append_one_token_with_heads_first_and_unaligned_rows():
+    gen = torch.Generator().manual_seed(4)
+    k = torch.randn(3, 1, 128, generator=gen).bfloat16().to(DEV).transpose(0, 1)
+    run_append([70], [1], 3, k, k, empty_cache(4, 3, 1), [[2, 0]])
+    flat = torch.randn(20 * 3 * 128 + 1, generator=gen).bfloat16().to(DEV)
+    k = flat[1:].view(20, 3, 128)
+    run_append([60], [20], 3, k, -k, empty_cache(4, 3, 1), [[2, 0]])
+
+
 def test_append_skips_tokens_without_pages_and_bad_pages():
     gen = torch.Generator().manual_seed(2)
     k = torch.randn(130, 1, 128, generator=gen).bfloat16().to(DEV)

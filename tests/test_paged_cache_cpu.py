@@ -169,6 +169,21 @@ def test_cpu_tensors_raise():
                        1, 1)
 
 
+def test_token_rows_are_laid_out_for_the_kernel():
+    """Rows the kernel cannot take as they stand are copied, also where torch calls them
+    contiguous: one token with its heads first, rows that begin off a 16-byte boundary."""
+    heads_first = torch.randn(4, 1, 128).bfloat16().transpose(0, 1)
+    odd = torch.randn(3 * 4 * 128 + 1).bfloat16()[1:].view(3, 4, 128)
+    spread = torch.randn(3, 4, 256).bfloat16()[..., ::2]
+    same = torch.zeros(1, 4, 128).bfloat16().expand(3, 4, 128)
+    for t in (heads_first, odd, spread, same, heads_first.float()):
+        rows = ops._token_rows(t)
+        assert rows.dtype == torch.bfloat16 and torch.equal(rows, t.bfloat16())
+        assert rows.stride() == (4 * 128, 128, 1) and rows.data_ptr() % 16 == 0
+    fused = torch.randn(3, 1024).bfloat16()[:, 512:].view(3, 4, 128)
+    assert ops._token_rows(fused) is fused
+
+
 def test_oracle_rounding_is_that_of_torch():
     """Every representable value, every midpoint between two and its neighbours."""
     codes = torch.arange(127, dtype=torch.uint8).view(torch.float8_e4m3fn).double()
