@@ -89,9 +89,15 @@ class PagedKVCache:
     def step(self, new_lens: Sequence[int]):
         """:meth:`plan` for a step that may fail on its way through the layers.
 
-        When the block raises, the cache holds the tokens it held before (rows
-        already written lie behind its lengths, and the next plan takes the
-        same pages).
+        When the block raises, the cache holds the tokens it held before: lengths,
+        pages and free list are taken back, rows already written lie behind the
+        lengths, and the next plan takes the same pages.  What is not taken back:
+        where a layer had written into a half-filled page before the step failed,
+        that page's scale may have grown for the new rows, as it would have in a
+        step that succeeds.  It stays, and older values below 2^-6 of it have been
+        rounded again, by at most 2^-10 of the scale.  (Rows with infinities raise
+        it to 2^48 and leave nothing of them: a caller that checks for those does
+        so before the write.)
         """
         before = self.seq_lens, self.free_head, self.lengths, self.taken, self.rope_len
         try:

@@ -1140,6 +1140,54 @@ def test_model_decode_refusals(model):
     assert cache.lengths == [64] and cache.taken == 1
 
 
+@pytest.mark.parametrize("size", [0.5, 1000.0, 1e6, math.inf])
+def test_a_failed_step_keeps_only_the_scale_it_raised(size):
+    """A step fails after its rows were written into a half-filled page: lengths and pages
+    are the old ones, older values moved by no more than the rounding to a scale that grew,
+    and the next step, with other rows, is the oracle's over what the page holds now."""
+    from leanselect_b200 import PagedKVCache
+
+    gen = torch.Generator().manual_seed(8)
+
+    def rows(n, scale=1.0):
+        return (torch.randn(n, 2, 128, generator=gen) * scale).bfloat16().to(DEV)
+
+    cache = PagedKVCache(1, 1, 192, 3, 2, device=DEV)
+    with cache.step([104]) as plan:
+        ops.append_kv(rows(104), rows(104), plan, *cache.layer(0))
+    layer, page = cache.layer(0), int(cache.block_table[0, 1])
+    before = [(as_values(layer[i])[page, :, :40], layer[2 + i][page].double().cpu())
+              for i in range(2)]
+    first = [t[cache.block_table[0, 0]].clone() for t in layer]
+    with pytest.raises(RuntimeError, match="a later layer"):
+        with cache.step([30]) as plan:
+            ops.append_kv(rows(30, size), rows(30, size), plan, *layer)
+            raise RuntimeError("a later layer")
+    assert cache.lengths == [104] and cache.seq_lens.tolist() == [104] and cache.taken == 2
+    assert cache.free_head.tolist() == [2]
+    for a, t in zip(first, layer):  # full pages as they were
+        assert torch.equal(a.view(torch.uint8), t[cache.block_table[0, 0]].view(torch.uint8))
+    for i, (codes, old) in enumerate(before):
+        now = layer[2 + i][page].double().cpu()
+        assert bool((now >= old).all()) and (size > 1 or torch.equal(now, old))
+        x = codes * old[:, None, None]
+        y = as_values(layer[i])[page, :, :40] * now[:, None, None]
+        assert bool(((x - y).abs() <= 2.0 ** -10 * now[:, None, None]).all())
+        normal = x.abs() >= 2.0 ** -6 * now[:, None, None]
+        assert torch.equal(x[normal], y[normal])
+    mirror = [as_values(layer[0]), as_values(layer[1]), layer[2].double().cpu(),
+              layer[3].double().cpu()]
+    k, v = rows(1), rows(1)
+    with cache.step([1]) as plan:
+        ops.append_kv(k, v, plan, *layer)
+        table = cache.block_table.tolist()
+    ora.append(k.cpu(), [104], [1], table, mirror[0], mirror[2])
+    ora.append(v.cpu(), [104], [1], table, mirror[1], mirror[3])
+    for got, want in zip((as_values(layer[0]), as_values(layer[1]), layer[2].double().cpu(),
+                          layer[3].double().cpu()), mirror):
+        assert torch.equal(got.nan_to_num(1234.0), want.nan_to_num(1234.0))
+
+
 def test_failed_steps_leave_the_cache_as_it_was(model):
     """A prefill and a decode step that raise between layers, then the same steps again."""
     from leanselect_b200 import PagedKVCache
