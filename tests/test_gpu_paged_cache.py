@@ -329,6 +329,28 @@ def test_append_offsets_that_are_no_prefix_sums_are_reported():
         ops.status_word(DEV).zero_()
 
 
+@pytest.mark.parametrize("cu_blocks, reported", [
+    ([5] * 100 + [7], True),               # blocks before the first request's
+    ([0] * 50 + [90] * 50 + [8], True),    # more than the total
+    (list(range(100, -1, -1)), False),     # a total of none: nothing to write
+])
+def test_append_bad_offsets_write_to_no_page_without_a_slot(cu_blocks, reported):
+    """All slots are in page 0: whatever the offsets say, pages 1 and 2 are left alone."""
+    gen = torch.Generator().manual_seed(3)
+    cache = empty_cache(3, 1, 1)
+    before = [c.clone() for c in cache]
+    k = torch.randn(100, 1, 128, generator=gen).bfloat16().to(DEV)
+    plan = ops.PagePlan(i32([0] * 100), i32([1] * 100), i32(list(range(101))), i32(cu_blocks),
+                        torch.zeros(100, dtype=torch.int64, device=DEV), None)
+    ops.append_kv(k, k, plan, *cache)
+    if reported:
+        with pytest.raises(_native.LeanSelectError, match="SEQLENS"):
+            ops.check_status(DEV)
+    for a, b in zip(before, cache):
+        first = 0 if cu_blocks[-1] == 0 else 1
+        assert torch.equal(a.view(torch.uint8)[first:], b.view(torch.uint8)[first:])
+
+
 def test_append_extremes():
     """Zeros, subnormals, values at and next to 448 s, infinities and NaN."""
     gen = torch.Generator().manual_seed(5)
@@ -624,6 +646,51 @@ def test_lists_that_overlap_are_joined(kind, H, G):
     idx = torch.nn.functional.pad(idx, (0, 0, 0, 300), value=0)   # rows behind the last request
     for causal in (True, False):
         run_attend(H, G, seq, nq, idx=idx, causal=causal, seed=G, pad=300)
+
+
+@pytest.mark.parametrize("kind", ["ascending", "shuffled", "future"])
+def test_joined_lists_of_512_pages(kind):
+    """The longest request that lists are joined for, whose union fills the shared table;
+    ranges of more pages than one batch of a producer warp."""
+    seq, nq = [512 * PAGE], [400]
+    run_attend(2, 2, seq, nq, idx=page_lists(seq, nq, 2, 128, 6, kind), seed=6)
+
+
+@pytest.mark.parametrize("H, G, T, longest, most", [
+    (1, 1, 128, 21800, 8),    # tiles of 8 rows, 341 pages
+    (6, 2, 60, 6400, 9),      # tiles of 15 rows
+    (8, 1, 128, 5000, 5),     # two tokens of 8 heads
+])
+@pytest.mark.parametrize("batch", [20, 45])
+def test_joined_lists_of_many_requests(H, G, T, longest, most, batch):
+    """Requests of no, one and several tokens, found by warp and by the whole block."""
+    gen = torch.Generator().manual_seed(batch)
+    seq = [1 + int(longest * x ** 4) for x in torch.rand(batch, generator=gen).tolist()]
+    nq = torch.randint(0, most + 1, (batch,), generator=gen).tolist()
+    seq[3], nq[3], nq[4], nq[5], nq[6] = longest, most, 0, 1, most
+    idx = page_lists(seq, nq, G, T, 2, "repeats")
+    # rows behind the last request, for the work that joining is worth
+    pad = 9000 // (G * T)
+    idx = torch.nn.functional.pad(idx, (0, 0, 0, pad), value=0)
+    run_attend(H, G, seq, nq, idx=idx, seed=batch, pad=pad)
+
+
+def test_joined_lists_past_their_512_pages_are_passed_over_and_reported():
+    """max_seqlen_k that is no bound: pages from the 512th on are not attended to."""
+    H, length, n = 2, 515 * PAGE, 80
+    codes, scales, table = make_cache([length], H, 2)
+    gen = torch.Generator().manual_seed(2)
+    q = torch.randn(n, H, 128, generator=gen).bfloat16()
+    idx = page_lists([length], [n], H, 128, 2, "shuffled")
+    idx[:, :, 5] = 512 + torch.arange(n, dtype=torch.int32) % 3
+    got = ops.paged_attn(q.to(DEV), codes[0].to(DEV), codes[1].to(DEV), scales[0].to(DEV),
+                         scales[1].to(DEV), i32(table), i32([length]), i32([0, n]), n, 512 * PAGE,
+                         topk_idx=idx.to(DEV))
+    want, _, bounds = ora.attend(q, codes[0].float(), codes[1].float(), scales[0], scales[1], table,
+                                 [length], [0, n], torch.where(idx < 512, idx, -1))
+    assert bool(((got.double().cpu() - want).abs() <= tolerance(want, bounds, length)).all())
+    with pytest.raises(_native.LeanSelectError, match="PAGE_INDEX"):
+        ops.check_status(DEV)
 
 
 def test_long_requests_keep_single_lists():
