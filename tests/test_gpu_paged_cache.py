@@ -659,7 +659,7 @@ def test_joined_lists_of_512_pages(kind):
 @pytest.mark.parametrize("H, G, T, longest, most", [
     (1, 1, 128, 21800, 8),    # tiles of 8 rows, 341 pages
     (6, 2, 60, 6400, 9),      # tiles of 15 rows
-    (8, 1, 128, 5000, 5),     # two tokens of 8 heads
+    (8, 2, 128, 10800, 7),    # four tokens of 4 heads
 ])
 @pytest.mark.parametrize("batch", [20, 45])
 def test_joined_lists_of_many_requests(H, G, T, longest, most, batch):
