@@ -36,16 +36,18 @@
 //
 // Measured (CUDA-graph replays): 64 ragged requests up to 32768 tokens, 2 x 8
 // heads, 596 MB of codes: 101 us, 5.9 TB/s, 0.90 of the measured copy rate
-// (95 us with all arithmetic taken out).  One request of 131072 tokens, 2 x 16
-// heads, 67 MB: 23.6 us, of which the stream takes 9, launch and first page
-// 4.5, the rows' end 1.2 and the merge 5.  A chunk of 512 tokens with 67 listed
+// (95 us with all arithmetic taken out; called from Python on inputs that
+// change 115 us, 0.79).  One request of 131072 tokens, 2 x 16
+// heads, 67 MB: 23.5 us, of which the stream takes 9, launch and first page
+// 4.5, the rows' end 1.2 and the merge 5; the other 3.7 are not placed.  A chunk of 512 tokens with 67 listed
 // pages each, 2 x 16 heads, 16 MB cached: 174 us, 207 TFLOP/s, against 71 us
 // for the page copies alone and 64 us for the products at mma.sync's rate (8
 // cycles per m16n8k16 and SM quarter): two warps per quarter, each a chain of
 // ~2300 cycles a page (wait 280, scores 620, softmax 540, values 500, the rest
 // bookkeeping), keep the tensor pipe 40 % busy.  Tried and dropped there: three teams
-// at 152 registers (152 us, but 5 us more for one long request), the next
-// page's scores formed beside this page's product with V (168-186 us).
+// at 152 registers (noted at 152 us in one form, 224 in another that was measured
+// again; one long request 4 to 9 us slower), the next page's scores formed beside
+// this page's product with V (168-186 us).
 #include <cuda_fp16.h>
 
 #include "common.cuh"
@@ -1262,7 +1264,10 @@ cudaError_t launch_attn_kernel(const PagedAttnArgs& args, int ranges, cudaStream
   ranges = ctas * kTeams;
   // More than 16 parts a row: by row.  2 rows of 131072 keys 23.4 us (by range
   // 49.8), 8 rows of 65536 34.3 (38.2), 16 rows of 32768 34.1 (34.1), 64 listed
-  // rows 34.4 (24.8).
+  // rows 34.4 (24.8).  All four are tiles of one token: the rule counts tokens,
+  // so tiles of several go by range with up to `pack` times as many parts a row
+  // (32 tokens of 2 x 1 heads over 131072 keys take 47 us that way; the other
+  // side was not measured).
   if (rows * 16 < ranges)
     return launch_early(paged_merge_many_kernel, dim3(static_cast<unsigned>(rows), heads),
                         dim3(32 * kMergeWarps), 0, stream, args, ranges);

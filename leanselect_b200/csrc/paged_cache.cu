@@ -439,6 +439,8 @@ cudaError_t launch_append_kv(const AppendArgs& args, cudaStream_t stream) {
   const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(args.num_groups));
   // Up to two tokens a request on average: single warps (512 tokens of 512
   // requests 2.8 us against 7.4; a prompt of 131072 tokens 57 us against 35).
+  // Idle requests count: a prompt of 16384 tokens beside 8191 of them takes the
+  // single warps, 35 us, where alone it takes 6.
   return args.total_new <= 2 * static_cast<int64_t>(args.batch)
              ? launch_early(append_kv_kernel<32>, grid, dim3(64), 0, stream, args)
              : launch_early(append_kv_kernel<128>, grid, dim3(256), 0, stream, args);
