@@ -871,11 +871,11 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
         }
         x0 = fmaf(x0, k0, v_log2);
         if (!kHalf) x1 = fmaf(x1, k1, v_log2);
-        if (__any_sync(0xffffffffu, x0 > m0 + kSlack || (!kHalf && x1 > m1 + kSlack))) {
+        if (__any_sync(0xffffffffu, x0 - m0 > kSlack || (!kHalf && x1 - m1 > kSlack))) {
           x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, 1));
           x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, 2));
           float a0 = 1.f, a1 = 1.f;
-          if (x0 > m0 + kSlack) {
+          if (x0 - m0 > kSlack) {
             a0 = ex2(m0 - (x0 - kHeadroom));
             m0 = x0 - kHeadroom;
           }
@@ -883,7 +883,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
           if (!kHalf) {
             x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, 1));
             x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, 2));
-            if (x1 > m1 + kSlack) {
+            if (x1 - m1 > kSlack) {
               a1 = ex2(m1 - (x1 - kHeadroom));
               m1 = x1 - kHeadroom;
             }
@@ -899,19 +899,22 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
             }
           }
         }
-        const float d0 = v_log2 - (m0 == -INFINITY ? 0.f : m0);
-        const float d1 = v_log2 - (m1 == -INFINITY ? 0.f : m1);
+        // Subtracted after the rounding that the maximum has seen too: scores whose
+        // last bit is worth binades (beyond 2^24) still give weights in f16's range.
+        const float r0 = m0 == -INFINITY ? 0.f : m0, r1 = m1 == -INFINITY ? 0.f : m1;
         float sum0 = 0.f, sum1 = 0.f;
         uint32_t pa[2][4];
 #pragma unroll
         for (int n = 0; n < 4; ++n) {
-          const float p0 = ex2(fmaf(sc[n][0], k0, d0)), p1 = ex2(fmaf(sc[n][1], k0, d0));
+          const float p0 = ex2(fmaf(sc[n][0], k0, v_log2) - r0);
+          const float p1 = ex2(fmaf(sc[n][1], k0, v_log2) - r0);
           sum0 += p0 + p1;
           pa[n >> 1][2 * (n & 1)] = pack_f16x2(p0, p1);
           if (kHalf) {
             pa[n >> 1][2 * (n & 1) + 1] = 0;
           } else {
-            const float p2 = ex2(fmaf(sc[n][2], k1, d1)), p3 = ex2(fmaf(sc[n][3], k1, d1));
+            const float p2 = ex2(fmaf(sc[n][2], k1, v_log2) - r1);
+            const float p3 = ex2(fmaf(sc[n][3], k1, v_log2) - r1);
             sum1 += p2 + p3;
             pa[n >> 1][2 * (n & 1) + 1] = pack_f16x2(p2, p3);
           }

@@ -562,6 +562,34 @@ def test_scales_and_peaked_rows(sizes, qsize):
     run_attend(32, 2, [700, 100], [2, 1], sizes=sizes, qsize=qsize, seed=4)
 
 
+@pytest.mark.parametrize("power", [40, 47, 50, 60, 78])
+@pytest.mark.parametrize("n", [1, 4])
+def test_scores_of_any_size(power, n):
+    """Scores far beyond 2^24, whose last bit is worth binades: queries along one key each,
+    so that the row is that key's value (every other key scores a quarter less)."""
+    H, length = 4, 300
+    codes, scales, table = make_cache([length], 1, 9)
+    gen = torch.Generator().manual_seed(power)
+    signs = torch.randint(0, 2, (up(length), PAGE, 128), generator=gen).double() * 2 - 1
+    for j, page in enumerate(table[0]):
+        codes[0][page, 0] = signs[j].float().to(FP8)
+        scales[0][page] = 2.0 ** -20
+    at = [17, 64, 130, 255][:n]
+    flat = signs.reshape(-1, 128)
+    # products with the other keys are at most 128 - 2 * 16
+    assert all(int((flat[:length] @ flat[a]).topk(2).values[1]) <= 96 for a in at)
+    q = torch.stack([flat[a] for a in at])[:, None].expand(n, H, 128) * 2.0 ** power
+    got, lse = ops.paged_attn(
+        q.bfloat16().contiguous().to(DEV), codes[0].to(DEV), codes[1].to(DEV), scales[0].to(DEV),
+        scales[1].to(DEV), i32(table), i32([length]), i32([0, n]), n, length, return_lse=True)
+    for i, a in enumerate(at):
+        page, row = table[0][a // PAGE], a % PAGE
+        want = codes[1][page, 0, row].double() * float(scales[1][page, 0])
+        assert torch.equal(got[i].double().cpu(), want.expand(H, 128))
+        score = 128 * 2.0 ** (power - 20) / math.sqrt(128)
+        assert bool(((lse[:, i].double().cpu() - score).abs() <= 2.0 ** -20 * score).all())
+
+
 def test_pages_of_very_different_value_scales():
     """A row whose weight sits in a page of tiny values next to pages of large ones."""
     gen = torch.Generator().manual_seed(6)
