@@ -252,8 +252,9 @@ __device__ __forceinline__ void load_query(const PagedAttnArgs& args, int token,
     amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
     amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
     // The exponent is kept to where the factor stays normal under every page
-    // scale.
-    const int e = min(max(static_cast<int>(__float_as_uint(amax) >> 23) - 127, -60), 78);
+    // scale, as far as the row's largest value then fits f16 (below 2^15).
+    const int top = static_cast<int>(__float_as_uint(amax) >> 23) - 127;
+    const int e = min(max(top, -60), max(78, top - 14));
     const float down = __int_as_float((127 - e) << 23);
     const float factor = args.scale_log2 * __int_as_float((127 + e) << 23);
     if (half == 0) *f0 = factor; else *f1 = factor;

@@ -590,6 +590,12 @@ def test_scores_of_any_size(power, n):
         assert bool(((lse[:, i].double().cpu() - score).abs() <= 2.0 ** -20 * score).all())
 
 
+@pytest.mark.parametrize("power", [93, 94, 110, 127])
+def test_queries_up_to_the_largest(power):
+    """bf16 queries beyond f16's range under their scaling: along one key each, as above."""
+    test_scores_of_any_size(power, 4)
+
+
 def test_pages_of_very_different_value_scales():
     """A row whose weight sits in a page of tiny values next to pages of large ones."""
     gen = torch.Generator().manual_seed(6)
