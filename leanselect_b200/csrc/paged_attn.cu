@@ -256,7 +256,10 @@ __device__ __forceinline__ void load_query(const PagedAttnArgs& args, int token,
     const int top = static_cast<int>(__float_as_uint(amax) >> 23) - 127;
     const int e = min(max(top, -60), max(78, top - 14));
     const float down = __int_as_float((127 - e) << 23);
-    const float factor = args.scale_log2 * __int_as_float((127 + e) << 23);
+    // Nor does a tiny softmax scale take it to 0, which times the -inf of a masked
+    // key would be NaN: products of 2^17 make at most 2^-21 of it.
+    const float factor =
+        fmaxf(args.scale_log2 * __int_as_float((127 + e) << 23), 0x1p-86f);
     if (half == 0) *f0 = factor; else *f1 = factor;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {

@@ -596,6 +596,15 @@ def test_queries_up_to_the_largest(power):
     test_scores_of_any_size(power, 4)
 
 
+@pytest.mark.parametrize("scale, qsize", [(1e-30, 0.0), (1e-20, 0.0), (1e-38, 1.5), (1e-42, 1.5),
+                                          (0.1, 0.0), (0.1, 1e-30)])
+def test_scores_next_to_zero(scale, qsize):
+    """Softmax scales and queries so small that their product with a key's scale
+    underflows: the weights are equal, masked keys stay out."""
+    run_attend(16, 2, [200, 70, 1], [1, 3, 1], scale=scale, qsize=qsize)
+    run_attend(16, 1, [9000], [1], scale=scale, qsize=qsize)
+
+
 def test_pages_of_very_different_value_scales():
     """A row whose weight sits in a page of tiny values next to pages of large ones."""
     gen = torch.Generator().manual_seed(6)
